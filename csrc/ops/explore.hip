@@ -511,8 +511,8 @@ __global__ __launch_bounds__(256) void explore_postprocess_oct_kernel(const floa
 #pragma unroll
     for (int k = 0; k < 8; ++k) wf[k] = explore_apply(wf[k], 0.f, v[k], 1, rand_mu, rand_sigma);
   } else {
-    // explore_apply on weight pairs: 2 mu - 1 (+ rand_mu) + sigma z as packed FMAs (v_pk_fma_f32, the same
-    // per-element IEEE operations), then fma(0.5, ., 0.5) with the clamp modifier per element: 4 VALU per pair
+    // explore_apply on weight pairs: 2 mu - 1 (+ rand_mu) + sigma z as pairs of FMAs (scalar instructions: the
+    // build has no packed fp32), then fma(0.5, ., 0.5) with the clamp modifier per element
     typedef float f2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
