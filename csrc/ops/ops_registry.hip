@@ -11,6 +11,9 @@ void register_replay(py::module_& m);
 void register_gnn_lw(py::module_& m);
 void register_actor_proj(py::module_& m);
 void register_sparse_act(py::module_& m);
+void register_norm(py::module_& m);
+void register_dropout(py::module_& m);
+void register_gated(py::module_& m);
 void register_ops(py::module_& m) {
   register_explore(m);
   register_gnn(m);
@@ -21,5 +24,8 @@ void register_ops(py::module_& m) {
   register_gnn_lw(m);
   register_actor_proj(m);
   register_sparse_act(m);
+  register_norm(m);
+  register_dropout(m);
+  register_gated(m);
 }
 }  // namespace gsc

@@ -1,0 +1,137 @@
+"""Gated linear layer (``csrc/ops/gated.hip``), forward and backward.
+
+    h = act(x Wg^T + bg) * (x Wu^T + bu)        weight [2F, D]: Wg rows over Wu rows, bias [2F]: bg, bu
+
+``gated_linear`` runs both projections, the activation and the product in one HIP kernel for CUDA tensors, and
+:func:`gated_linear_reference` otherwise.  Operands are bf16 or fp32 with fp32 accumulation; nothing but ``x`` is kept for
+the backward pass, which recomputes both projections and takes every derivative from fp32 values.
+
+* bf16 ``x`` with fp32 masters: the weight operand is the masters' bf16 shadow (``FlatParams``) or a cast; their gradients
+  come back in fp32.  Under autocast fp32 ``x`` is cast the same way, like :func:`gsc_amd.ops.linear.linear`.
+* fp32 ``x`` and weight outside autocast: fp32 matrix instructions.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from gsc_amd.native import load as load_native
+from .linear import shadow
+from .norm import _TYPES, check_cuda, device_guard, note_leaves, rows_of
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
+
+
+def gated_linear_reference(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                           activation: str = "silu") -> torch.Tensor:
+    """The same function in PyTorch operations (fp32 inside, fp64 for fp64 inputs), differentiable."""
+    dt = torch.float64 if x.dtype == torch.float64 else torch.float32
+    g, u = F.linear(x.to(dt), weight.to(dt), bias.to(dt) if bias is not None else None).chunk(2, -1)
+    a = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid}[activation](g)
+    return (a * u).to(x.dtype)
+
+
+def _p(t) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
+def _bf(t) -> bool:
+    return t is not None and t.dtype == torch.bfloat16
+
+
+def _forward(x2, w, bias, act):
+    M, D = x2.shape
+    Fo = w.shape[0] // 2
+    h = torch.empty(M, Fo, device=x2.device, dtype=x2.dtype)
+    if M > 0:
+        with device_guard(x2):
+            load_native().gated_forward(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _bf(x2), _p(bias), _bf(bias),
+                                        h.data_ptr(), M, D, Fo, act, torch.cuda.current_stream(x2.device).cuda_stream)
+    return h
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, w, act, dtype):
+        x2 = rows_of(x, x.shape[-1]).to(dtype)
+        h = _forward(x2, w, bias, act)
+        ctx.save_for_backward(x2, w, bias)
+        ctx.act, ctx.x, ctx.w_dtype = act, (x.shape, x.dtype), weight.dtype
+        return h.view(*x.shape[:-1], h.shape[1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        x2, w, bias = ctx.saved_tensors
+        (M, D), Fo = x2.shape, w.shape[0] // 2
+        shape, x_dtype = ctx.x
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        mk = lambda *s, dt: torch.empty(*s, device=x2.device, dtype=dt)
+        dx = mk(M, D, dt=x_dtype) if need_x else None
+        dw = mk(2 * Fo, D, dt=ctx.w_dtype) if need_w else None
+        db = mk(2 * Fo, dt=bias.dtype) if need_b else None
+        if M == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        else:
+            nat = load_native()
+            dh2 = rows_of(dh, Fo).to(x2.dtype)
+            dgu = mk(M, 2 * Fo, dt=x2.dtype)
+            part = mk(nat.gated_bias_workspace(M, Fo), dt=torch.float32) if need_b else None
+            with device_guard(x2):
+                s = torch.cuda.current_stream(x2.device).cuda_stream
+                nat.gated_backward_pair(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _bf(x2), _p(bias), _bf(bias),
+                                        dh2.data_ptr(), dh2.stride(0), dgu.data_ptr(), _p(part), _p(db), _bf(db), M, D, Fo,
+                                        ctx.act, s)
+                if need_x:
+                    nat.gated_backward_x(dgu.data_ptr(), w.data_ptr(), w.stride(0), _bf(x2), dx.data_ptr(), _bf(dx), M, D,
+                                         Fo, s)
+                if need_w:
+                    nat.gated_backward_w(dgu.data_ptr(), x2.data_ptr(), x2.stride(0), _bf(x2), dw.data_ptr(), _bf(dw), M, D,
+                                         Fo, s)
+        return dx.view(shape) if need_x else None, dw, db, None, None, None
+
+
+def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "silu",
+                 w16: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """See the module docstring.  ``x`` [.., D] -> [.., F]; ``activation``: silu, gelu (exact, erf) or sigmoid.  ``w16``:
+    the bf16 weight operand of fp32 masters (default: their ``FlatParams`` shadow, else a cast)."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"gated_linear: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"gated_linear: x needs a last dimension of at least 1, got shape {tuple(x.shape)}")
+    D = x.shape[-1]
+    if weight.dim() != 2 or weight.shape[1] != D or weight.shape[0] % 2 or weight.shape[0] == 0:
+        raise ValueError(f"gated_linear: weight must be [2F, {D}], got {tuple(weight.shape)}")
+    if bias is not None and bias.shape != (weight.shape[0],):
+        raise ValueError(f"gated_linear: bias must have shape ({weight.shape[0]},), got {tuple(bias.shape)}")
+    if w16 is not None and (w16.shape != weight.shape or w16.dtype != torch.bfloat16):
+        raise ValueError(f"gated_linear: w16 must be bfloat16 {tuple(weight.shape)}, got {w16.dtype} {tuple(w16.shape)}")
+    if not x.is_cuda:
+        return gated_linear_reference(x, weight, bias, activation)
+    for k, t in (("x", x), ("weight", weight), ("bias", bias)):
+        if t is not None and t.dtype not in _TYPES:
+            raise TypeError(f"gated_linear: {k} must be bfloat16 or float32 on the GPU, got {t.dtype}")
+    check_cuda("gated_linear", x, weight=weight, bias=bias, w16=w16)
+    dtype = x.dtype
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        if dtype != torch.bfloat16:
+            raise TypeError(f"gated_linear: autocast to {dtype} is not supported (bfloat16)")
+    if dtype == torch.float32 and weight.dtype != torch.float32:
+        raise TypeError("gated_linear: float32 x needs a float32 weight")
+    w = weight
+    if weight.dtype != dtype:
+        w = w16 if w16 is not None else shadow(weight)
+        w = w if w is not None else weight.detach().to(dtype)
+    w = rows_of(w.detach(), D)
+    bias = bias.contiguous() if bias is not None else None
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        h = _GatedLinear.apply(x, weight, bias, w, ACTIVATIONS[activation], dtype)
+        return note_leaves("gated_linear", h, x, weight, bias)
+    h = _forward(rows_of(x, D).to(dtype), w, bias, ACTIVATIONS[activation])
+    return h.view(*x.shape[:-1], h.shape[1])
