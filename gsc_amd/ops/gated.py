@@ -42,8 +42,22 @@ def _bf(t) -> bool:
     return t is not None and t.dtype == torch.bfloat16
 
 
-def _forward(x2, w, bias, act):
-    M, D = x2.shape
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """The matrix [rows, cols] as the kernels read it: bf16 rows start on 16 bytes and end on a multiple of 8 elements
+    (a copy with zeros behind each row where they do not)."""
+    rows, cols = t.shape
+    if t.dtype != torch.bfloat16 or rows == 0 or (cols % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+                                                  and t.stride(0) >= cols):
+        return t
+    out = torch.empty(rows, -(-cols // 8) * 8, device=t.device, dtype=t.dtype)
+    with device_guard(t):
+        load_native().gated_pad(t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0), True, rows, cols,
+                                torch.cuda.current_stream(t.device).cuda_stream)
+    return out
+
+
+def _forward(x2, w, bias, act, D):
+    M = x2.shape[0]
     Fo = w.shape[0] // 2
     h = torch.empty(M, Fo, device=x2.device, dtype=x2.dtype)
     if M > 0:
@@ -56,8 +70,9 @@ def _forward(x2, w, bias, act):
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, w, act, dtype):
-        x2 = rows_of(x, x.shape[-1]).to(dtype)
-        h = _forward(x2, w, bias, act)
+        D = x.shape[-1]
+        x2, w = _operand(rows_of(x, D).to(dtype)), _operand(w)
+        h = _forward(x2, w, bias, act, D)
         ctx.save_for_backward(x2, w, bias)
         ctx.act, ctx.x, ctx.w_dtype = act, (x.shape, x.dtype), weight.dtype
         return h.view(*x.shape[:-1], h.shape[1])
@@ -66,8 +81,8 @@ class _GatedLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh):
         x2, w, bias = ctx.saved_tensors
-        (M, D), Fo = x2.shape, w.shape[0] // 2
         shape, x_dtype = ctx.x
+        M, D, Fo = x2.shape[0], shape[-1], w.shape[0] // 2
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         mk = lambda *s, dt: torch.empty(*s, device=x2.device, dtype=dt)
         dx = mk(M, D, dt=x_dtype) if need_x else None
@@ -80,8 +95,10 @@ class _GatedLinear(torch.autograd.Function):
         else:
             nat = load_native()
             dh2 = rows_of(dh, Fo).to(x2.dtype)
-            dgu = mk(M, 2 * Fo, dt=x2.dtype)
-            part = mk(nat.gated_bias_workspace(M, Fo), dt=torch.float32) if need_b else None
+            half = -(-Fo // 8) * 8 if _bf(x2) else Fo
+            dgu = mk(M, 2 * half, dt=x2.dtype)
+            part = mk(nat.gated_bias_workspace(_bf(x2), M, Fo), dt=torch.float32) if need_b else None
+            slabs = mk(nat.gated_weight_workspace(_bf(x2), M, D, Fo), dt=torch.float32) if need_w else None
             with device_guard(x2):
                 s = torch.cuda.current_stream(x2.device).cuda_stream
                 nat.gated_backward_pair(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _bf(x2), _p(bias), _bf(bias),
@@ -91,8 +108,8 @@ class _GatedLinear(torch.autograd.Function):
                     nat.gated_backward_x(dgu.data_ptr(), w.data_ptr(), w.stride(0), _bf(x2), dx.data_ptr(), _bf(dx), M, D,
                                          Fo, s)
                 if need_w:
-                    nat.gated_backward_w(dgu.data_ptr(), x2.data_ptr(), x2.stride(0), _bf(x2), dw.data_ptr(), _bf(dw), M, D,
-                                         Fo, s)
+                    nat.gated_backward_w(dgu.data_ptr(), x2.data_ptr(), x2.stride(0), _bf(x2), dw.data_ptr(), _bf(dw),
+                                         slabs.data_ptr(), M, D, Fo, s)
         return dx.view(shape) if need_x else None, dw, db, None, None, None
 
 
@@ -133,5 +150,5 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         h = _GatedLinear.apply(x, weight, bias, w, ACTIVATIONS[activation], dtype)
         return note_leaves("gated_linear", h, x, weight, bias)
-    h = _forward(rows_of(x, D).to(dtype), w, bias, ACTIVATIONS[activation])
+    h = _forward(_operand(rows_of(x, D).to(dtype)), _operand(w), bias, ACTIVATIONS[activation], D)
     return h.view(*x.shape[:-1], h.shape[1])
