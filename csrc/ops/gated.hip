@@ -1,11 +1,11 @@
 // Gated linear layer h = act(x Wg^T + bg) * (x Wu^T + bu) and its gradients (gfx950, MFMA, fp32 accumulation).
 //
 //   weight [2F][D] = Wg over Wu, bias [2F] = bg, bu;  act: silu g s(g), gelu g Phi(g), sigmoid s(g)
-//   forward     g, u per 64 x 64 tile in one kernel; act, product and rounding in its epilogue
-//   backward    g, u again (nothing but x is kept), dg = dh u act'(g), du = dh act(g) from the fp32 accumulators,
+//   forward     both products of a tile in one kernel; bias, activation, product and rounding in its epilogue
+//   backward    g and u again (nothing but x is kept), dg = dh u act'(g), du = dh act(g) from the fp32 accumulators,
 //               rounded once to the operand type;  dx = dg Wg + du Wu,  dW = [dg | du]^T x,  db = column sums (fp32)
 //
-// T = bf16 runs on v_mfma_f32_32x32x16_bf16, T = float on v_mfma_f32_32x32x2_f32.
+// bf16 operands run on v_mfma_f32_32x32x16_bf16, fp32 on v_mfma_f32_32x32x2_f32.
 #include <hip/hip_bf16.h>
 #include <algorithm>
 #include <pybind11/pybind11.h>
@@ -17,26 +17,39 @@ namespace py = pybind11;
 namespace gsc {
 namespace gated {
 
+typedef __hip_bfloat16 bf16;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
-typedef __hip_bfloat16 bf16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) char lds_char;
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
-template <class T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ bf16 from_f<bf16>(float v) { return __float2bfloat16(v); }
+__device__ __forceinline__ float to_f(short v) { return __bfloat162float(__builtin_bit_cast(bf16, v)); }
+__device__ __forceinline__ short to_s(float v) { return __builtin_bit_cast(short, __float2bfloat16(v)); }
+
+// ---- activations
 
 enum Act { SILU = 0, GELU = 1, SIGMOID = 2 };
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + __expf(-g)); }
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+
+// Phi(g) = (1 + erf(g / sqrt 2)) / 2 and e = exp(-g^2 / 2), by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7):
+// the exponential is the one the derivative needs.
+__device__ __forceinline__ float normal_cdf(float g, float& e) {
+  e = __expf(-0.5f * g * g);
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(g));
+  const float q = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * q * e;
+  return g < 0.f ? tail : 1.f - tail;
+}
 
 __device__ __forceinline__ float act_fwd(int act, float g) {
-  if (act == GELU) return g * (0.5f + 0.5f * erff(g * 0.70710678f));
+  float e;
+  if (act == GELU) return g * normal_cdf(g, e);
   const float s = sigmoid(g);
   return act == SILU ? g * s : s;
 }
@@ -44,61 +57,15 @@ __device__ __forceinline__ float act_fwd(int act, float g) {
 // a = act(g), d = act'(g)
 __device__ __forceinline__ void act_both(int act, float g, float& a, float& d) {
   if (act == GELU) {
-    const float phi = 0.5f + 0.5f * erff(g * 0.70710678f);
+    float e;
+    const float phi = normal_cdf(g, e);
     a = g * phi;
-    d = phi + g * __expf(-0.5f * g * g) * 0.39894228f;
+    d = phi + g * e * 0.39894228f;
     return;
   }
   const float s = sigmoid(g);
   a = act == SILU ? g * s : s;
   d = act == SILU ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
-}
-
-// One operand, element (r, k) at p[r sr + k sk].
-template <class T>
-struct Mat {
-  const T* p;
-  long sr, sk;
-};
-
-template <class T>
-struct Tile;  // LDS image of 64 rows x BK, and the products of one BK step
-template <>
-struct Tile<bf16> {
-  static constexpr int BK = 32, LD = 40;  // 80-byte rows
-  static __device__ __forceinline__ void mul(const bf16* a, const bf16* b, int lane, f32x16& c) {
-    const int r = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int s = 0; s < BK / 16; ++s)
-      c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(a + r * LD + 16 * s + 8 * h),
-                                                  *reinterpret_cast<const bf16x8*>(b + r * LD + 16 * s + 8 * h), c, 0, 0, 0);
-  }
-};
-template <>
-struct Tile<float> {
-  static constexpr int BK = 16, LD = 20;
-  static __device__ __forceinline__ void mul(const float* a, const float* b, int lane, f32x16& c) {
-    const int r = lane & 31, h = lane >> 5;
-    // a lane's four floats are k = 8 s + 4 h ..: product t takes k = 8 s + t and 8 s + 4 + t of both operands
-#pragma unroll
-    for (int s = 0; s < BK / 8; ++s) {
-      const f32x4 fa = *reinterpret_cast<const f32x4*>(a + r * LD + 8 * s + 4 * h);
-      const f32x4 fb = *reinterpret_cast<const f32x4*>(b + r * LD + 8 * s + 4 * h);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[t], fb[t], c, 0, 0, 0);
-    }
-  }
-};
-
-template <class T>
-__device__ __forceinline__ void stage(const Mat<T>& m, long r0, long rows, long k0, long K, T* img) {
-  constexpr int BK = Tile<T>::BK, LD = Tile<T>::LD;
-  for (int i = threadIdx.x; i < 64 * BK; i += 256) {
-    // neighbouring threads take neighbouring elements of the operand's contiguous dimension
-    const int r = m.sk == 1 ? i / BK : i % 64, k = m.sk == 1 ? i % BK : i / 64;
-    const bool in = r0 + r < rows && k0 + k < K;
-    img[r * LD + k] = in ? m.p[(r0 + r) * m.sr + (k0 + k) * m.sk] : from_f<T>(0.f);
-  }
 }
 
 struct Bias {
@@ -111,126 +78,52 @@ struct Bias {
 };
 
 // Row of accumulator register r of lane: v_mfma 32x32 C layout (the column is lane & 31).
-__device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
-
-// BWD 0: h[m][f].  BWD 1: dgu[m][f] = dg, dgu[m][F + f] = du, and part[2 * tile + wave row][0 .. 2F) = their column sums.
-template <class T, int BWD>
-__global__ __launch_bounds__(256) void pair_kernel(Mat<T> x, Mat<T> w, Bias bias, const T* dh, long lddh, T* out, float* part,
-                                                   long M, long D, long F, int act) {
-  constexpr int IMG = 64 * Tile<T>::LD;
-  __shared__ __attribute__((aligned(16))) T img[3 * IMG];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  const long m0 = (long)blockIdx.x * 64, f0 = (long)blockIdx.y * 64;
-  const Mat<T> wu{w.p + F * w.sr, w.sr, w.sk};
-  f32x16 g, u;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) g[r] = u[r] = 0.f;
-  for (long k0 = 0; k0 < D; k0 += Tile<T>::BK) {
-    stage(x, m0, M, k0, D, img);
-    stage(w, f0, F, k0, D, img + IMG);
-    stage(wu, f0, F, k0, D, img + 2 * IMG);
-    __syncthreads();
-    const T* a = img + wm * 32 * Tile<T>::LD;
-    Tile<T>::mul(a, img + IMG + wn * 32 * Tile<T>::LD, lane, g);
-    Tile<T>::mul(a, img + 2 * IMG + wn * 32 * Tile<T>::LD, lane, u);
-    __syncthreads();
-  }
-  const long f = f0 + wn * 32 + (lane & 31);
-  const float bg = f < F ? bias.at(f) : 0.f, bu = f < F ? bias.at(F + f) : 0.f;
-  float sg = 0.f, su = 0.f;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const long m = m0 + wm * 32 + acc_row(r, lane);
-    if (m >= M || f >= F) continue;
-    const float gv = g[r] + bg, uv = u[r] + bu;
-    if (!BWD) {
-      out[m * F + f] = from_f<T>(act_fwd(act, gv) * uv);
-    } else {
-      float a, d;
-      act_both(act, gv, a, d);
-      const float dv = to_f(dh[m * lddh + f]);
-      const float dg = dv * uv * d, du = dv * a;
-      out[m * 2 * F + f] = from_f<T>(dg);
-      out[m * 2 * F + F + f] = from_f<T>(du);
-      sg += dg;
-      su += du;
-    }
-  }
-  if (BWD && part) {
-    sg += __shfl_xor(sg, 32);
-    su += __shfl_xor(su, 32);
-    if (lane < 32 && f < F) {
-      float* row = part + (2 * (long)blockIdx.x + wm) * 2 * F;
-      row[f] = sg;
-      row[F + f] = su;
-    }
-  }
-}
-
-// out[r][c] = sum_k A(r, k) B(c, k), rounded once to the output type.
-template <class T>
-__global__ __launch_bounds__(256) void prod_kernel(Mat<T> a, Mat<T> b, void* out, int out_bf, long ldo, long R, long C, long K) {
-  constexpr int IMG = 64 * Tile<T>::LD;
-  __shared__ __attribute__((aligned(16))) T img[2 * IMG];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  const long r0 = (long)blockIdx.x * 64, c0 = (long)blockIdx.y * 64;
-  f32x16 acc;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-  for (long k0 = 0; k0 < K; k0 += Tile<T>::BK) {
-    stage(a, r0, R, k0, K, img);
-    stage(b, c0, C, k0, K, img + IMG);
-    __syncthreads();
-    Tile<T>::mul(img + wm * 32 * Tile<T>::LD, img + IMG + wn * 32 * Tile<T>::LD, lane, acc);
-    __syncthreads();
-  }
-  const long c = c0 + wn * 32 + (lane & 31);
-  if (c >= C) return;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const long row = r0 + wm * 32 + acc_row(r, lane);
-    if (row >= R) continue;
-    if (out_bf) reinterpret_cast<bf16*>(out)[row * ldo + c] = __float2bfloat16(acc[r]);
-    else reinterpret_cast<float*>(out)[row * ldo + c] = acc[r];
-  }
-}
-
-// out[c] = sum over the partial rows, in a fixed order.
-__global__ __launch_bounds__(256) void colsum_kernel(const float* part, long rows, long C, void* out, int out_bf) {
-  const long c = (long)blockIdx.x * 256 + threadIdx.x;
-  if (c >= C) return;
-  float s = 0.f;
-  for (long z = 0; z < rows; ++z) s += part[z * C + c];
-  if (out_bf) reinterpret_cast<bf16*>(out)[c] = __float2bfloat16(s);
-  else reinterpret_cast<float*>(out)[c] = s;
-}
-
+__device__ __forceinline__ constexpr int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// bf16 tiles.  out = sum_k A(r, k) B(c, k) on BM x BN tiles, K in steps of 64, both operands copied straight from
-// memory into LDS (buffer loads to LDS, 16 bytes a lane) one step ahead of the products.
+// Tiles.  out = sum_k A(r, k) B(c, k) on BM x BN tiles, K in steps of 128 bytes (64 bf16, 32 fp32), both operands copied
+// straight from memory into LDS (buffer loads to LDS, 16 bytes a lane) one step ahead of the products.
 //
-//   row operand (k contiguous)   LDS [R][64], 16-byte chunk c of row r in slot c ^ ((r >> 1) & 7): the 16 rows of a
-//                                fragment read cover all 64 banks once
-//   column operand (r contiguous) LDS [64][R], chunk c of row k in slot c ^ 4 (k & 3): the four rows of a transposing
-//                                read (ds_read_b64_tr_b16) fall on four different 64-byte quarters of the banks
+//   row operand (k contiguous)    LDS [R][128 B], 16-byte chunk c of row r in slot c ^ ((r >> 1) & 7): the 16 rows of a
+//                                 fragment read cover all 64 banks once
+//   column operand (r contiguous) LDS [k][R]; bf16: chunk c of row k in slot c ^ 4 (k & 3), so the four rows of a
+//                                 transposing read (ds_read_b64_tr_b16) fall on four different quarters of the banks;
+//                                 fp32: slot c ^ 8 ((k >> 2) & 1), so the two halves of a wave read different banks
 // The copy to LDS writes lane l's 16 bytes at 16 l, so the slots are permuted on the address side.  Rows and chunks
 // outside the matrices get an offset past the buffer descriptor's end: the load returns zeros.  Operands are 16-byte
 // aligned with rows of a multiple of 8 elements (the caller pads others), so a chunk is inside or outside as a whole.
 
 constexpr unsigned kOut = 0x80000000u;   // past every descriptor (2^31 - 1 bytes)
-typedef __attribute__((address_space(3))) short lds_short;
-typedef __attribute__((ext_vector_type(4))) short s16x4;
-typedef __attribute__((ext_vector_type(8))) short s16x8;
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-template <int R, int WAVES, bool COL>
+template <class T>
+struct Elem;
+template <>
+struct Elem<bf16> {
+  static constexpr int STEP = 64, CHUNK = 8;   // k per step, elements per 16 bytes
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ f32x16 mma(const frag& a, const frag& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Elem<float> {
+  static constexpr int STEP = 32, CHUNK = 4;
+  typedef f32x4 frag;   // a lane's k = 8 s + 4 half ..: product t takes element t, k = 8 s + t and 8 s + 4 + t
+  static __device__ __forceinline__ f32x16 mma(const frag& a, const frag& b, f32x16 c) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <class T, int R, int WAVES, bool COL>
 struct Copy {
   static constexpr int PER = R / 8 / WAVES;   // 1 KB wave copies per wave and step
+  static constexpr int CH = Elem<T>::CHUNK;
   static_assert(R % (8 * WAVES) == 0 && (!COL || R == 128 || R == 256), "tile");
   unsigned off[PER];
   int kk[PER];      // k (row operand: of the chunk's first element; column operand: of the row) inside a step
-  unsigned step;    // bytes per step
+  long step;        // elements per step
   // r0: first row (column) of the tile, rows: their count in the matrix, ld: elements between stored rows
   __device__ __forceinline__ void init(long r0, long rows, long ld, int wave, int lane) {
 #pragma unroll
@@ -238,73 +131,80 @@ struct Copy {
       const int q = i * WAVES + wave;
       if (!COL) {
         const int r = 8 * q + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-        off[i] = r0 + r < rows ? (unsigned)(r * ld * 2 + 16 * c) : kOut;
-        kk[i] = 8 * c;
+        off[i] = r0 + r < rows ? (unsigned)(r * ld * sizeof(T) + 16 * c) : kOut;
+        kk[i] = CH * c;
       } else {
-        constexpr int CPR = R / 8;   // chunks per stored row
-        const int k = q * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ ((k & 3) << 2);
-        off[i] = r0 + 8 * c < rows ? (unsigned)(k * ld * 2 + 16 * c) : kOut;
+        constexpr int CPR = R / CH;   // chunks per stored row
+        const int k = q * 64 / CPR + lane / CPR;
+        const int c = (lane % CPR) ^ (CH == 8 ? (k & 3) << 2 : ((k >> 2) & 1) << 3);
+        off[i] = r0 + CH * c < rows ? (unsigned)(k * ld * sizeof(T) + 16 * c) : kOut;
         kk[i] = k;
       }
     }
-    step = COL ? (unsigned)(64 * ld * 2) : 128u;
+    step = COL ? Elem<T>::STEP * ld : Elem<T>::STEP;
   }
-  // base: the tile's first element at this step, left: k that remain (>= 64: all)
-  __device__ __forceinline__ void load(const bf16* base, long left, short* img, int wave) const {
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, 0x7fffffff, 0x00027000);
+  // base: the tile's first element at this step, left: k that remain (>= a step: all)
+  __device__ __forceinline__ void load(const T* base, long left, T* img, int wave) const {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, 0x7fffffff, 0x00027000);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const unsigned o = left >= 64 || kk[i] < left ? off[i] : kOut;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_short*)(img + 512 * (i * WAVES + wave)), 16, o, 0, 0, 0);
+      const unsigned o = left >= Elem<T>::STEP || kk[i] < left ? off[i] : kOut;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_char*)((char*)img + 1024 * (i * WAVES + wave)), 16, o, 0, 0, 0);
     }
   }
 };
 
-// Addresses of a wave's 32 x 16 fragments in an image of R rows (columns).  Fragment i covers rows r0 + 32 i; r0 is a
-// multiple of 32 N for column images.  Everything but one register per k step (row image) or per fragment (column image)
-// is an immediate offset of the read.
-template <int R, bool COL, int N>
+// Addresses of a wave's 32-row fragments in an image of R rows (columns).  Fragment i covers rows r0 + 32 i.  Everything
+// but one register per k step (row image) or per fragment (column image) is an immediate offset of the read.
+template <class T, int R, bool COL, int N>
 struct Frags {
-  const short* at[COL ? N : 4];
-  __device__ __forceinline__ void init(const short* img, int r0, int lane) {
+  static constexpr int STEP = Elem<T>::STEP, CH = Elem<T>::CHUNK;
+  typedef typename Elem<T>::frag frag;
+  const T* at[COL ? N : 4];
+  __device__ __forceinline__ void init(const T* img, int r0, int lane) {
     if constexpr (!COL) {
       const int r = r0 + (lane & 31), c = (lane >> 5) ^ ((r >> 1) & 7);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) at[s] = img + r * 64 + 8 * (c ^ (2 * s));
-    } else {
+      for (int s = 0; s < 4; ++s) at[s] = img + r * STEP + CH * (c ^ (2 * s));
+    } else if constexpr (CH == 8) {
       const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
 #pragma unroll
       for (int i = 0; i < N; ++i)
         at[i] = img + (8 * (g >> 1) + q) * R + 8 * ((((r0 >> 3) + 4 * i) ^ (q << 2)) + 2 * (g & 1) + (p >> 1)) + 4 * (p & 1);
+    } else {
+      const int h = lane >> 5;
+#pragma unroll
+      for (int i = 0; i < N; ++i) at[i] = img + 4 * h * R + ((r0 + 32 * i + (lane & 31)) ^ (h << 5));
     }
   }
-  // fragment i of k step s; shift: elements to the image in use
-  __device__ __forceinline__ bf16x8 read(int i, int s, int shift) const {
+  // fragment i of quarter s of the step; shift: elements to the image in use
+  __device__ __forceinline__ frag read(int i, int s, int shift) const {
     if constexpr (!COL) {
-      return *reinterpret_cast<const bf16x8*>(at[s] + shift + 32 * 64 * i);
-    } else {
-      const short* a = at[i] + shift + 16 * s * R;
+      return *reinterpret_cast<const frag*>(at[s] + shift + 32 * STEP * i);
+    } else if constexpr (CH == 8) {
+      const T* a = at[i] + shift + 16 * s * R;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * R));
-      return __builtin_bit_cast(bf16x8, (s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}));
+      return __builtin_bit_cast(frag, (s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}));
+    } else {
+      const T* a = at[i] + shift + 8 * s * R;
+      return frag{a[0], a[R], a[2 * R], a[3 * R]};
     }
   }
 };
 
 struct TileArgs {
-  const bf16* a[2];   // operands of the two K segments (dx: gate and up halves), one segment otherwise
-  const bf16* b[2];   // pair kernels: gate and up rows instead
+  const void* a[2];   // operands of the two K segments (dx: gate and up halves), one segment otherwise
+  const void* b[2];   // pair kernels: gate and up rows instead
   long lda, ldb;
   int segs;
   long M, N, K;       // rows, columns (pair: F) and K of a segment
   int tm, tn;         // tiles
   long kchunk;        // K of a split (whole steps; one segment only), K otherwise
   Bias bias;
-  const bf16* dh;
+  const void* dh;
   long lddh;
   void* out;
-  int out_bf;
   long ldo;
   long half;          // dgu: column of du
   long slab;          // elements between the fp32 partial results of two splits
@@ -323,51 +223,89 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& pm, int& pn
   pn = (t % width) / rows;
 }
 
-enum Epi { FWD = 0, BWD = 1, OUT = 2 };
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
-template <int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
+// Sum over the 32 lanes of each half wave, in its lane 31 (DPP adds in a fixed order).
+__device__ __forceinline__ float half_wave_sum(float v) {
+#define GSC_ADD_DPP(ctrl, mask)                                                                                      \
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, mask, 0xf, true))
+  GSC_ADD_DPP(0x111, 0xf);   // row_shr 1, 2, 4, 8: lane 15 of each 16 holds their sum
+  GSC_ADD_DPP(0x112, 0xf);
+  GSC_ADD_DPP(0x114, 0xf);
+  GSC_ADD_DPP(0x118, 0xf);
+  GSC_ADD_DPP(0x142, 0xa);   // row_bcast 15 into rows 1 and 3
+#undef GSC_ADD_DPP
+  return v;
+}
+
+// What leaves a tile: FWD h, BWD dgu (and the bias gradient's partial sums), OUT the product in T, SUM in fp32 (split
+// partial results, gradients of fp32 masters).
+enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3 };
+
+// bf16 tiles swap the operands of the matrix instruction, so that a lane holds four neighbouring columns of one row and
+// stages them in LDS with one 8-byte write; fp32 results leave from the accumulators as 128-byte row pieces.
+template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
-  constexpr int WAVES = WM * WN, BM = 32 * RM * WM, BN = 32 * RN * WN;
-  constexpr bool PAIR = EPI != OUT;
+  typedef Elem<T> E;
+  constexpr int WAVES = WM * WN, NT = 64 * WAVES, BM = 32 * RM * WM, BN = 32 * RN * WN;
+  constexpr bool PAIR = EPI == FWD || EPI == BWD, SWAP = E::CHUNK == 8 && EPI != SUM;
   constexpr int BH = PAIR ? BN / 2 : BN;            // columns of one product
   constexpr int SH = PAIR ? RN / 2 : RN;            // 32-column fragments of one product per wave
-  constexpr int ASZ = BM * 64, BSZ = BN * 64;
+  constexpr int ASZ = BM * E::STEP, BSZ = BN * E::STEP, OPS = 2 * (ASZ + BSZ) * (int)sizeof(T);
   constexpr int OC = EPI == FWD ? BH : BN, OLD = OC + 8;   // output columns of the tile, staged row stride
-  constexpr int OPS = 2 * (ASZ + BSZ), STG = BM * OLD;
-  __shared__ __attribute__((aligned(1024))) short smem[OPS > STG ? OPS : STG];
+  constexpr int STG = SWAP ? BM * OLD * 2 : 0;
+  __shared__ __attribute__((aligned(1024))) char smem[OPS > STG ? OPS : STG];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int pm, pn;
   tile_of(blockIdx.x, g.tm, g.tn, pm, pn);
-  const int up = EPI == OUT && g.tmh && pm >= g.tmh;   // dW: rows of the up half
+  const int up = !PAIR && g.tmh && pm >= g.tmh;   // dW: rows of the up half
+  const int part_row = pm * WM + wm;
   if (up) pm -= g.tmh;
   const long m0 = (long)pm * BM, n0 = (long)pn * BH;
   const long k0 = (long)blockIdx.y * g.kchunk, kend = k0 + g.kchunk < g.K ? k0 + g.kchunk : g.K;
-  const int steps = (int)((kend - k0 + 63) / 64), total = steps * g.segs;
+  const int steps = (int)((kend - k0 + E::STEP - 1) / E::STEP), total = steps * g.segs;
 
   // two images of each operand: A0 A1 | B0 B1
-  short *const ia = smem, *const ib = smem + 2 * ASZ;
-  Copy<BM, WAVES, ACOL> ca;
-  Copy<BH, WAVES, BCOL> cb;
+  T *const ia = reinterpret_cast<T*>(smem), *const ib = ia + 2 * ASZ;
+  Copy<T, BM, WAVES, ACOL> ca;
+  Copy<T, BH, WAVES, BCOL> cb;
   ca.init(m0, g.M, g.lda, wave, lane);
   cb.init(n0, g.N, g.ldb, wave, lane);
   const long a0 = (ACOL ? m0 + k0 * g.lda : m0 * g.lda + k0) + up * g.half, b0 = BCOL ? n0 + k0 * g.ldb : n0 * g.ldb + k0;
   auto load = [&](int t, int buf) {
     const int seg = t >= steps ? 1 : 0, st = t - seg * steps;
-    const long left = kend - k0 - 64L * st;
-    ca.load(g.a[PAIR ? 0 : seg] + a0 + (long)st * (ca.step / 2), left, ia + buf * ASZ, wave);
-    const long bo = b0 + (long)st * (cb.step / 2);
+    const long left = kend - k0 - (long)E::STEP * st;
+    ca.load(reinterpret_cast<const T*>(g.a[PAIR ? 0 : seg]) + a0 + st * ca.step, left, ia + buf * ASZ, wave);
+    const long bo = b0 + st * cb.step;
     if (PAIR) {
-      cb.load(g.b[0] + bo, left, ib + buf * BSZ, wave);
-      cb.load(g.b[1] + bo, left, ib + buf * BSZ + BH * 64, wave);
+      cb.load(reinterpret_cast<const T*>(g.b[0]) + bo, left, ib + buf * BSZ, wave);
+      cb.load(reinterpret_cast<const T*>(g.b[1]) + bo, left, ib + buf * BSZ + BH * E::STEP, wave);
     } else {
-      cb.load(g.b[seg] + bo, left, ib + buf * BSZ, wave);
+      cb.load(reinterpret_cast<const T*>(g.b[seg]) + bo, left, ib + buf * BSZ, wave);
     }
   };
-  Frags<BM, ACOL, RM> fa_at;
-  Frags<BH, BCOL, SH> fb_at;
+  Frags<T, BM, ACOL, RM> fa_at;
+  Frags<T, BH, BCOL, SH> fb_at;
   fa_at.init(ia, 32 * wm * RM, lane);
   fb_at.init(ib, 32 * wn * SH, lane);
+
+  // bf16 backward: the tile of dh waits in registers behind the products
+  constexpr int DPT = EPI == BWD && SWAP ? BM * BH / 8 / NT : 1;
+  s16x8 dh[DPT];
+  if constexpr (EPI == BWD && SWAP) {
+#pragma unroll
+    for (int q = 0; q < DPT; ++q) {
+      const int idx = q * NT + tid, row = idx / (BH / 8), c = idx % (BH / 8) * 8;
+      dh[q] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (m0 + row < g.M && n0 + c < g.N)
+        dh[q] = *reinterpret_cast<const s16x8*>(reinterpret_cast<const short*>(g.dh) + (m0 + row) * g.lddh + n0 + c);
+    }
+  }
 
   f32x16 acc[RM][RN];
 #pragma unroll
@@ -377,127 +315,185 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  auto step = [&](int t, int buf) {
-    // this step's copies have landed and every wave has read the other images
+  typename E::frag fa[2][RM], fb[2][RN];
+  auto read = [&](int s, int buf) {
+#pragma unroll
+    for (int i = 0; i < RM; ++i) fa[s & 1][i] = fa_at.read(i, s, buf * ASZ);
+#pragma unroll
+    for (int j = 0; j < RN; ++j) fb[s & 1][j] = fb_at.read(j % SH, s, buf * BSZ + (j / SH) * BH * E::STEP);
+  };
+  auto mul = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+      for (int j = 0; j < RN; ++j)
+        acc[i][j] = SWAP ? E::mma(fb[s & 1][j], fa[s & 1][i], acc[i][j]) : E::mma(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+  };
+  // The next step's copies have landed and every wave has taken its last fragments of this one: its images are free.
+  auto turn = [&] {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (t + 1 < total) load(t + 1, buf ^ 1);
+  };
+  // Fragments are read one quarter ahead of the products, across the steps too, so the matrix cores have work while
+  // the waves meet at the barrier.
+  auto step = [&](int t, int buf) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      bf16x8 fa[RM], fb[RN];
-#pragma unroll
-      for (int i = 0; i < RM; ++i) fa[i] = fa_at.read(i, s, buf * ASZ);
-#pragma unroll
-      for (int j = 0; j < RN; ++j) fb[j] = fb_at.read(j % SH, s, buf * BSZ + (j / SH) * BH * 64);
-#pragma unroll
-      for (int i = 0; i < RM; ++i)
-#pragma unroll
-        for (int j = 0; j < RN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+    for (int s = 0; s < 3; ++s) {
+      read(s + 1, buf);
+      mul(s);
     }
+    if (t + 1 < total) {
+      turn();
+      if (t + 2 < total) load(t + 2, buf);
+      read(0, buf ^ 1);
+    }
+    mul(3);
   };
   load(0, 0);
+  turn();
+  if (total > 1) load(1, 1);
+  read(0, 0);
   for (int t = 0; t < total; t += 2) {
     step(t, 0);
     if (t + 1 < total) step(t + 1, 1);
   }
 
   // ---- epilogue
-  const int cl = lane & 31;
-  if constexpr (EPI == OUT) {
-    if (!g.out_bf) {   // fp32: 128-byte row pieces straight from the accumulators
-      const int row0 = 32 * wm * RM + 4 * (lane >> 5);
-#pragma unroll 1
-      for (int j = 0; j < SH; ++j) {
-        const long n = n0 + 32 * (wn * SH + j) + cl;
-        float* o = reinterpret_cast<float*>(g.out) + blockIdx.y * g.slab + (m0 + row0 + up * g.M) * g.ldo + n;
-        const long left = n < g.N ? g.M - m0 - row0 : 0;
+  if constexpr (!SWAP) {
+    const int row0 = 32 * wm * RM + 4 * (lane >> 5);
+    const long left = g.M - m0 - row0;
 #pragma unroll
-        for (int i = 0; i < RM; ++i)
+    for (int j = 0; j < SH; ++j) {
+      const long n = n0 + 32 * (wn * SH + j) + (lane & 31);
+      const bool in = n < g.N;
+      float* o = reinterpret_cast<float*>(g.out) + blockIdx.y * g.slab + (m0 + row0 + up * g.M) * g.ldo + n;
+      const float* dv = EPI == BWD ? reinterpret_cast<const float*>(g.dh) + (m0 + row0) * g.lddh + n : nullptr;
+      const float bg = PAIR && in ? g.bias.at(n) : 0.f, bu = PAIR && in ? g.bias.at(g.N + n) : 0.f;
+      float sg = 0.f, su = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int row = 32 * i + acc_row(r, 0);
-            float v = acc[i][0][r];
+      for (int i = 0; i < RM; ++i)
 #pragma unroll
-            for (int q = 1; q < SH; ++q) v = j == q ? acc[i][q][r] : v;
-            if (row < left) *o = v;
-            o += (r == 15 ? 32 * (i + 1) - row : acc_row(r + 1, 0) - acc_row(r, 0)) * g.ldo;
-          }
-      }
-      return;
-    }
-  }
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();   // the operand images are free
-#pragma unroll
-  for (int j = 0; j < SH; ++j) {
-    const int col = 32 * (wn * SH + j) + cl;
-    const long n = n0 + col;
-    float bg = 0.f, bu = 0.f, sg = 0.f, su = 0.f;
-    if (PAIR && n < g.N) {
-      bg = g.bias.at(n);
-      bu = g.bias.at(g.N + n);
-    }
-#pragma unroll
-    for (int i = 0; i < RM; ++i) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = 32 * (wm * RM + i) + acc_row(r, lane);
-        const long m = m0 + row;
-        if constexpr (EPI == OUT) {
-          smem[row * OLD + col] = __builtin_bit_cast(short, __float2bfloat16(acc[i][j][r]));
-        } else {
-          const float gv = acc[i][j][r] + bg, uv = acc[i][j + SH][r] + bu;
-          if constexpr (EPI == FWD) {
-            smem[row * OLD + col] = __builtin_bit_cast(short, __float2bfloat16(act_fwd(g.act, gv) * uv));
-          } else {
-            float dg = 0.f, du = 0.f;
-            if (m < g.M && n < g.N) {
+        for (int r = 0; r < 16; ++r) {
+          const int row = 32 * i + acc_row(r, 0), next = r == 15 ? 32 * (i + 1) : 32 * i + acc_row(r + 1, 0);
+          if (in && row < left) {
+            if constexpr (EPI == BWD) {
               float a, d;
-              act_both(g.act, gv, a, d);
-              const float dv = to_f(g.dh[m * g.lddh + n]);
-              dg = dv * uv * d;
-              du = dv * a;
+              act_both(g.act, acc[i][j][r] + bg, a, d);
+              const float u = acc[i][j + SH][r] + bu;
+              const float dg = *dv * u * d, du = *dv * a;
+              o[0] = dg;
+              o[g.half] = du;
+              sg += dg;
+              su += du;
+            } else if constexpr (EPI == FWD) {
+              *o = act_fwd(g.act, acc[i][j][r] + bg) * (acc[i][j + SH][r] + bu);
+            } else {
+              *o = acc[i][j][r];
             }
-            smem[row * OLD + col] = __builtin_bit_cast(short, __float2bfloat16(dg));
-            smem[row * OLD + BH + col] = __builtin_bit_cast(short, __float2bfloat16(du));
-            sg += dg;
-            su += du;
+          } else if (EPI == BWD && n >= g.N && n < g.half && row < left) {
+            o[0] = o[g.half] = 0.f;   // the padding is an operand of dx
+          }
+          o += (next - row) * g.ldo;
+          if (EPI == BWD) dv += (next - row) * g.lddh;
+        }
+      if (EPI == BWD && g.part) {
+        sg += __shfl_xor(sg, 32);
+        su += __shfl_xor(su, 32);
+        if (lane < 32 && in) {
+          g.part[(long)part_row * 2 * g.N + n] = sg;
+          g.part[(long)part_row * 2 * g.N + g.N + n] = su;
+        }
+      }
+    }
+    return;
+  } else {
+    short* stage = reinterpret_cast<short*>(smem);
+    lds_barrier();   // the operand images are free
+    if constexpr (EPI == BWD) {
+#pragma unroll
+      for (int q = 0; q < DPT; ++q) {
+        const int idx = q * NT + tid, row = idx / (BH / 8), c = idx % (BH / 8) * 8;
+        *reinterpret_cast<s16x8*>(stage + row * OLD + c) = dh[q];
+      }
+      lds_barrier();
+    }
+#pragma unroll
+    for (int j = 0; j < SH; ++j) {
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg) {
+        const int col = 32 * (wn * SH + j) + 8 * rg + 4 * (lane >> 5);   // this lane's four columns
+        float bg[4], bu[4], sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
+        if (PAIR) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const long n = n0 + col + e;
+            bg[e] = n < g.N ? g.bias.at(n) : 0.f;
+            bu[e] = n < g.N ? g.bias.at(g.N + n) : 0.f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < RM; ++i) {
+          short* p = stage + (32 * (wm * RM + i) + (lane & 31)) * OLD + col;
+          s16x4 v, w;
+          if constexpr (EPI == BWD) w = *reinterpret_cast<const s16x4*>(p);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float c = acc[i][j][4 * rg + e];
+            if constexpr (EPI == OUT) {
+              v[e] = to_s(c);
+            } else if constexpr (EPI == FWD) {
+              v[e] = to_s(act_fwd(g.act, c + bg[e]) * (acc[i][j + SH][4 * rg + e] + bu[e]));
+            } else {
+              // rows and columns outside have dh = 0
+              float a, d;
+              act_both(g.act, c + bg[e], a, d);
+              const float x = to_f((short)w[e]);
+              const float dg = x * (acc[i][j + SH][4 * rg + e] + bu[e]) * d, du = x * a;
+              v[e] = to_s(dg);
+              w[e] = to_s(du);
+              sg[e] += dg;
+              su[e] += du;
+            }
+          }
+          *reinterpret_cast<s16x4*>(p) = v;
+          if constexpr (EPI == BWD) *reinterpret_cast<s16x4*>(p + BH) = w;
+        }
+        if (EPI == BWD && g.part) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = half_wave_sum(sg[e]), b = half_wave_sum(su[e]);
+            const long n = n0 + col + e;
+            if ((lane & 31) == 31 && n < g.N) {
+              g.part[(long)part_row * 2 * g.N + n] = a;
+              g.part[(long)part_row * 2 * g.N + g.N + n] = b;
+            }
           }
         }
       }
     }
-    if (EPI == BWD && g.part) {
-      sg += __shfl_xor(sg, 32);
-      su += __shfl_xor(su, 32);
-      if (lane < 32 && n < g.N) {
-        float* row = g.part + ((long)pm * WM + wm) * 2 * g.N;
-        row[n] = sg;
-        row[g.N + n] = su;
+    lds_barrier();
+    // rows of the staged tile leave in 16-byte pieces; dgu rows are padded to whole pieces (with zeros), others may end
+    // inside one or start off 16 bytes
+    const long cols = EPI == BWD ? g.half : g.N;
+    bf16* out = reinterpret_cast<bf16*>(g.out);
+    const bool vec = ((uintptr_t)out % 16 == 0) && g.ldo % 8 == 0;
+    for (int idx = tid; idx < BM * (OC / 8); idx += NT) {
+      const int row = idx / (OC / 8), c = idx % (OC / 8) * 8;
+      const long m = m0 + row, n = n0 + (EPI == BWD ? c % BH : c);
+      if (m >= g.M || n >= cols) continue;
+      const short* src = stage + row * OLD + c;
+      bf16* dst = out + (m + up * g.M) * g.ldo + n + (EPI == BWD && c >= BH ? g.half : 0);
+      if (vec && n + 8 <= cols) {
+        *reinterpret_cast<s16x8*>(dst) = *reinterpret_cast<const s16x8*>(src);
+      } else {
+        for (int e = 0; e < 8 && n + e < cols; ++e) dst[e] = __builtin_bit_cast(bf16, src[e]);
       }
     }
   }
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  // rows of the staged tile leave in 16-byte pieces; dgu rows are padded to whole pieces (with zeros), others may end
-  // inside one or start off 16 bytes
-  const long cols = EPI == BWD ? g.half : g.N;
-  bf16* out = reinterpret_cast<bf16*>(g.out);
-  const bool vec = ((uintptr_t)out % 16 == 0) && g.ldo % 8 == 0;
-  for (int idx = tid; idx < BM * (OC / 8); idx += 64 * WAVES) {
-    const int row = idx / (OC / 8), c = idx % (OC / 8) * 8;
-    const long m = m0 + row, n = n0 + (EPI == BWD ? c % BH : c);
-    if (m >= g.M || n >= cols) continue;
-    const short* src = smem + row * OLD + c;
-    bf16* dst = out + (m + up * g.M) * g.ldo + n + (EPI == BWD && c >= BH ? g.half : 0);
-    if (vec && n + 8 <= cols) {
-      *reinterpret_cast<s16x8*>(dst) = *reinterpret_cast<const s16x8*>(src);
-    } else {
-      for (int e = 0; e < 8 && n + e < cols; ++e) dst[e] = __builtin_bit_cast(bf16, src[e]);
-    }
-  }
 }
+
+// ---------------------------------------------------------------------------------------------------------------
 
 // dst [rows][ldd]: the rows of src, zeros behind them.
 template <class T>
@@ -505,7 +501,7 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* src, long lds_, T* ds
   const long n = rows * ldd;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
     const long r = i / ldd, c = i - r * ldd;
-    dst[i] = c < cols ? src[r * lds_ + c] : from_f<T>(0.f);
+    dst[i] = c < cols ? src[r * lds_ + c] : T(0.f);
   }
 }
 
@@ -519,19 +515,36 @@ __global__ __launch_bounds__(256) void splits_kernel(const float* slabs, long sl
   }
 }
 
+// out[c] = sum over the partial rows: 16 columns x 16 row phases a workgroup, phases added in order.
+__global__ __launch_bounds__(256) void colsum_kernel(const float* part, long rows, long C, void* out, int out_bf) {
+  __shared__ float red[16][17];
+  const int cl = threadIdx.x & 15, ph = threadIdx.x >> 4;
+  const long c = (long)blockIdx.x * 16 + cl;
+  float s = 0.f;
+  if (c < C)
+    for (long z = ph; z < rows; z += 16) s += part[z * C + c];
+  red[ph][cl] = s;
+  __syncthreads();
+  if (ph || c >= C) return;
+#pragma unroll
+  for (int q = 1; q < 16; ++q) s += red[q][cl];
+  if (out_bf) reinterpret_cast<bf16*>(out)[c] = __float2bfloat16(s);
+  else reinterpret_cast<float*>(out)[c] = s;
+}
+
 static long up8(long n) { return (n + 7) / 8 * 8; }
-static unsigned tiles(long n, long t = 64) { return (unsigned)((n + t - 1) / t); }
+static long tiles(long n, long t) { return (n + t - 1) / t; }
 static unsigned flat_grid(long n) { return (unsigned)std::max<long>(1, std::min<long>((n + 255) / 256, 4096)); }
 
 static void check_sizes(long M, long D, long F, int act) {
-  GSC_CHECK(M >= 1 && D >= 1 && F >= 1 && M <= 0x7fffffffL && D <= 4000000L && F <= 4000000L,
-            "gated_linear: rows must be in 1 .. 2^31 - 1, D and F in 1 .. 4,000,000");
+  GSC_CHECK(M >= 1 && D >= 1 && F >= 1 && M <= 0x7fffffffL && D <= 1000000L && F <= 1000000L,
+            "gated_linear: rows must be in 1 .. 2^31 - 1, D and F in 1 .. 1,000,000");
   GSC_CHECK(act >= 0 && act <= 2, "gated_linear: unknown activation");
 }
 
-// Operands of the bf16 tiles: 16-byte aligned rows.
+// Operands of the tiles: 16-byte aligned rows; 256 of them within the 2^31 bytes of a descriptor.
 static void check_operand(uintptr_t p, long ld) {
-  GSC_CHECK(p % 16 == 0 && ld % 8 == 0 && ld <= 4000000L, "gated_linear: a bf16 operand needs 16-byte aligned rows");
+  GSC_CHECK(p % 16 == 0 && ld % 8 == 0 && ld <= 2000000L, "gated_linear: an operand needs 16-byte aligned rows of at most 2,000,000 elements");
 }
 
 static int cu_count() {
@@ -543,71 +556,58 @@ static int cu_count() {
   return n;
 }
 
-template <int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
+template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
 static void launch(TileArgs g, int splits, hipStream_t s) {
-  constexpr int BM = 32 * RM * WM, BH = EPI == OUT ? 32 * RN * WN : 16 * RN * WN;
-  g.tm = (int)tiles(g.M, BM);
-  g.tn = (int)tiles(g.N, BH);
-  if (g.tmh) {
-    g.tmh = g.tm;
-    g.tm *= 2;
-  }
-  GSC_CHECK((long)g.tm * g.tn <= 0x7fffffffL, "gated_linear: too many tiles");
-  hipLaunchKernelGGL((tile_kernel<RM, RN, WM, WN, ACOL, BCOL, EPI>), dim3((unsigned)(g.tm * g.tn), splits), dim3(64 * WM * WN),
-                     0, s, g);
+  constexpr int BM = 32 * RM * WM, BH = EPI == FWD || EPI == BWD ? 16 * RN * WN : 32 * RN * WN;
+  const long tm = tiles(g.M, BM), tn = tiles(g.N, BH);
+  GSC_CHECK(2 * tm * tn <= 0x7fffffffL, "gated_linear: too many tiles");
+  if (g.tmh) g.tmh = (int)tm;
+  g.tm = (int)(g.tmh ? 2 * tm : tm);
+  g.tn = (int)tn;
+  hipLaunchKernelGGL((tile_kernel<T, RM, RN, WM, WN, ACOL, BCOL, EPI>), dim3((unsigned)(g.tm * g.tn), splits),
+                     dim3(64 * WM * WN), 0, s, g);
   check_launch();
 }
 
 // 256-row tiles where they fill the CUs, 128-row tiles otherwise.
-static bool large(long M, long N, long bn) { return (long)tiles(M, 256) * tiles(N, bn) >= cu_count(); }
-
+static bool large(long M, long N, long bn) { return tiles(M, 256) * tiles(N, bn) >= cu_count(); }
 static int pair_rows(long M, long F) { return large(M, F, 128) ? 256 : 128; }
+// Partial rows of the bias gradient: two wave rows a tile.
+static long part_rows(long M, long F) { return 2 * tiles(M, pair_rows(M, F)); }
 
-template <int EPI>
-static void pair_bf16(TileArgs g, hipStream_t s) {
-  if (pair_rows(g.M, g.N) == 256) launch<4, 2, 2, 4, false, false, EPI>(g, 1, s);
-  else launch<2, 2, 2, 2, false, false, EPI>(g, 1, s);
+template <class T, int EPI>
+static void pair(const TileArgs& g, hipStream_t s) {
+  if (pair_rows(g.M, g.N) == 256) launch<T, 4, 2, 2, 4, false, false, EPI>(g, 1, s);
+  else launch<T, 2, 2, 2, 2, false, false, EPI>(g, 1, s);
 }
 
-template <class T, int BWD>
-static void pair(uintptr_t x, long ldx, uintptr_t w, long ldw, Bias b, uintptr_t dh, long lddh, uintptr_t out, uintptr_t part,
-                 long M, long D, long F, int act, hipStream_t s) {
-  hipLaunchKernelGGL((pair_kernel<T, BWD>), dim3(tiles(M), tiles(F)), dim3(256), 0, s, Mat<T>{ptr<const T>(x), ldx, 1},
-                     Mat<T>{ptr<const T>(w), ldw, 1}, b, ptr<const T>(dh), lddh, ptr<T>(out), ptr<float>(part), M, D, F, act);
-  check_launch();
-}
-
-static TileArgs pair_args(uintptr_t x, long ldx, uintptr_t w, long ldw, Bias b, long M, long D, long F, int act) {
+static TileArgs pair_args(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, long M, long D,
+                          long F, int act) {
+  check_sizes(M, D, F, act);
   check_operand(x, ldx);
   check_operand(w, ldw);
   TileArgs g{};
-  g.a[0] = ptr<const bf16>(x);
-  g.b[0] = ptr<const bf16>(w);
-  g.b[1] = g.b[0] + F * ldw;
+  g.a[0] = ptr<const void>(x);
+  g.b[0] = ptr<const void>(w);
+  g.b[1] = ptr<const void>(w + F * ldw * (bf ? 2 : 4));
   g.lda = ldx;
   g.ldb = ldw;
   g.segs = 1;
   g.M = M;
   g.N = F;
   g.K = g.kchunk = up8(D);   // rows are padded with zeros
-  g.bias = b;
+  g.bias = Bias{ptr<const void>(bias), bias_bf};
   g.act = act;
   return g;
 }
 
 void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h, long M, long D,
              long F, int act, uintptr_t stream) {
-  check_sizes(M, D, F, act);
-  const Bias b{ptr<const void>(bias), bias_bf};
-  const hipStream_t s = stream_of(stream);
-  if (!bf) {
-    pair<float, 0>(x, ldx, w, ldw, b, 0, 0, h, 0, M, D, F, act, s);
-    return;
-  }
-  TileArgs g = pair_args(x, ldx, w, ldw, b, M, D, F, act);
+  TileArgs g = pair_args(x, ldx, w, ldw, bf, bias, bias_bf, M, D, F, act);
   g.out = ptr<void>(h);
   g.ldo = F;
-  pair_bf16<FWD>(g, s);
+  if (bf) pair<bf16, FWD>(g, stream_of(stream));
+  else pair<float, FWD>(g, stream_of(stream));
 }
 
 void pad(uintptr_t src, long lds_, uintptr_t dst, long ldd, int bf, long rows, long cols, uintptr_t stream) {
@@ -619,65 +619,45 @@ void pad(uintptr_t src, long lds_, uintptr_t dst, long ldd, int bf, long rows, l
   check_launch();
 }
 
-// Elements of dgu rows: [dg, zeros to a multiple of 8 | du, zeros] for bf16, [dg | du] for fp32.
-static long half_of(int bf, long F) { return bf ? up8(F) : F; }
-
-static long part_rows(int bf, long M, long F) {
-  if (!bf) return 2L * tiles(M);
-  return 2L * tiles(M, pair_rows(M, F));
-}
-
 // fp32 elements of the bias gradient's partial sums.
-long bias_workspace(int bf, long M, long F) { return part_rows(bf, M, F) * 2 * F; }
+long bias_workspace(long M, long F) { return part_rows(M, F) * 2 * F; }
 
-// dgu from x, the weights and dh; part (absent: no bias gradient) takes the column sums' partial rows.
+// dgu rows [dg, zeros to a multiple of 8 | du, zeros] from x, the weights and dh; part (absent: no bias gradient) takes
+// the column sums' partial rows.
 void backward_pair(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t dh, long lddh,
                    uintptr_t dgu, uintptr_t part, uintptr_t db, int db_bf, long M, long D, long F, int act,
                    uintptr_t stream) {
-  check_sizes(M, D, F, act);
+  TileArgs g = pair_args(x, ldx, w, ldw, bf, bias, bias_bf, M, D, F, act);
   GSC_CHECK(!db || part, "gated_linear: the bias gradient needs a workspace");
-  const Bias b{ptr<const void>(bias), bias_bf};
+  if (bf) check_operand(dh, lddh);
   const hipStream_t s = stream_of(stream);
-  if (bf) {
-    TileArgs g = pair_args(x, ldx, w, ldw, b, M, D, F, act);
-    g.dh = ptr<const bf16>(dh);
-    g.lddh = lddh;
-    g.out = ptr<void>(dgu);
-    g.half = half_of(bf, F);
-    g.ldo = 2 * g.half;
-    g.part = db ? ptr<float>(part) : nullptr;
-    pair_bf16<BWD>(g, s);
-  } else {
-    pair<float, 1>(x, ldx, w, ldw, b, dh, lddh, dgu, db ? part : 0, M, D, F, act, s);
-  }
+  g.dh = ptr<const void>(dh);
+  g.lddh = lddh;
+  g.out = ptr<void>(dgu);
+  g.half = up8(F);
+  g.ldo = 2 * g.half;
+  g.part = db ? ptr<float>(part) : nullptr;
+  if (bf) pair<bf16, BWD>(g, s);
+  else pair<float, BWD>(g, s);
   if (db) {
-    hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)((2 * F + 255) / 256)), dim3(256), 0, s, ptr<const float>(part),
-                       part_rows(bf, M, F), 2 * F, ptr<void>(db), db_bf);
+    hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)tiles(2 * F, 16)), dim3(256), 0, s, ptr<const float>(part),
+                       part_rows(M, F), 2 * F, ptr<void>(db), db_bf);
     check_launch();
   }
-}
-
-template <class T>
-static void prod(Mat<T> a, Mat<T> b, uintptr_t out, int out_bf, long R, long C, long K, hipStream_t s) {
-  hipLaunchKernelGGL((prod_kernel<T>), dim3(tiles(R), tiles(C)), dim3(256), 0, s, a, b, ptr<void>(out), out_bf, C, R, C, K);
-  check_launch();
 }
 
 void backward_x(uintptr_t dgu, uintptr_t w, long ldw, int bf, uintptr_t dx, int dx_bf, long M, long D, long F,
                 uintptr_t stream) {
   check_sizes(M, D, F, 0);
   const hipStream_t s = stream_of(stream);
-  if (!bf) {
-    prod<float>({ptr<const float>(dgu), 2 * F, 1}, {ptr<const float>(w), 1, ldw}, dx, dx_bf, M, D, 2 * F, s);
-    return;
-  }
   check_operand(dgu, 2 * up8(F));
   check_operand(w, ldw);
+  const int es = bf ? 2 : 4;
   TileArgs g{};
-  g.a[0] = ptr<const bf16>(dgu);
-  g.a[1] = g.a[0] + up8(F);
-  g.b[0] = ptr<const bf16>(w);
-  g.b[1] = g.b[0] + F * ldw;
+  g.a[0] = ptr<const void>(dgu);
+  g.a[1] = ptr<const void>(dgu + up8(F) * es);
+  g.b[0] = ptr<const void>(w);
+  g.b[1] = ptr<const void>(w + F * ldw * es);
   g.lda = 2 * up8(F);
   g.ldb = ldw;
   g.segs = 2;
@@ -685,21 +665,30 @@ void backward_x(uintptr_t dgu, uintptr_t w, long ldw, int bf, uintptr_t dx, int 
   g.N = D;
   g.K = g.kchunk = F;
   g.out = ptr<void>(dx);
-  g.out_bf = dx_bf;
   g.ldo = D;
-  if (large(M, D, 256)) launch<4, 2, 2, 4, false, true, OUT>(g, 1, s);
-  else launch<2, 2, 2, 2, false, true, OUT>(g, 1, s);
+  const bool big = large(M, D, 256);
+  GSC_CHECK(bf || !dx_bf, "gated_linear: fp32 operands give fp32 gradients");
+  if (!bf) {
+    if (big) launch<float, 4, 2, 2, 4, false, true, SUM>(g, 1, s);
+    else launch<float, 2, 2, 2, 2, false, true, SUM>(g, 1, s);
+  } else if (dx_bf) {
+    if (big) launch<bf16, 4, 2, 2, 4, false, true, OUT>(g, 1, s);
+    else launch<bf16, 2, 2, 2, 2, false, true, OUT>(g, 1, s);
+  } else {
+    if (big) launch<bf16, 4, 2, 2, 4, false, true, SUM>(g, 1, s);
+    else launch<bf16, 2, 2, 2, 2, false, true, SUM>(g, 1, s);
+  }
 }
 
 // Splits of dW's reduction over the rows: enough workgroups for two per CU, at least 512 rows each.
 static int w_splits(long M, long D, long F) {
   if (large(2 * F, D, 256)) return 1;
-  const long t = 2L * tiles(F, 128) * tiles(D, 128);
+  const long t = 2 * tiles(F, 128) * tiles(D, 128);
   return (int)std::max<long>(1, std::min<long>({(2L * cu_count() + t - 1) / t, M / 512, 64}));
 }
 
-long w_workspace(int bf, long M, long D, long F) {
-  const int n = bf ? w_splits(M, D, F) : 1;
+long w_workspace(long M, long D, long F) {
+  const int n = w_splits(M, D, F);
   return n > 1 ? n * 2 * F * D : 0;
 }
 
@@ -707,38 +696,38 @@ void backward_w(uintptr_t dgu, uintptr_t x, long ldx, int bf, uintptr_t dw, int 
                 uintptr_t stream) {
   check_sizes(M, D, F, 0);
   const hipStream_t s = stream_of(stream);
-  if (!bf) {
-    prod<float>({ptr<const float>(dgu), 1, 2 * F}, {ptr<const float>(x), 1, ldx}, dw, dw_bf, 2 * F, D, M, s);
-    return;
-  }
   check_operand(dgu, 2 * up8(F));
   check_operand(x, ldx);
   const int splits = w_splits(M, D, F);
   GSC_CHECK(splits == 1 || slabs, "gated_linear: the weight gradient needs a workspace");
+  GSC_CHECK(bf || !dw_bf, "gated_linear: fp32 operands give fp32 gradients");
   TileArgs g{};
-  g.a[0] = ptr<const bf16>(dgu);
-  g.b[0] = ptr<const bf16>(x);
+  g.a[0] = ptr<const void>(dgu);
+  g.b[0] = ptr<const void>(x);
   g.lda = 2 * up8(F);
   g.ldb = ldx;
   g.segs = 1;
   g.M = F;
   g.N = D;
   g.K = M;
-  g.kchunk = (M + splits - 1) / splits;
-  g.kchunk = (g.kchunk + 63) / 64 * 64;
+  g.kchunk = tiles(tiles(M, splits), 64) * 64;
   g.half = up8(F);
   g.tmh = 1;
   g.ldo = D;
-  const int used = (int)((M + g.kchunk - 1) / g.kchunk);
-  if (splits > 1) {
-    g.out = ptr<void>(slabs);
-    g.slab = 2 * F * D;
+  g.slab = 2 * F * D;
+  g.out = ptr<void>(splits > 1 ? slabs : dw);
+  const int used = (int)tiles(M, g.kchunk);
+  const bool big = large(2 * F, D, 256), sum = splits > 1 || !dw_bf;
+  if (!bf) {
+    if (big) launch<float, 4, 2, 2, 4, true, true, SUM>(g, used, s);
+    else launch<float, 2, 2, 2, 2, true, true, SUM>(g, used, s);
+  } else if (sum) {
+    if (big) launch<bf16, 4, 2, 2, 4, true, true, SUM>(g, used, s);
+    else launch<bf16, 2, 2, 2, 2, true, true, SUM>(g, used, s);
   } else {
-    g.out = ptr<void>(dw);
-    g.out_bf = dw_bf;
+    if (big) launch<bf16, 4, 2, 2, 4, true, true, OUT>(g, used, s);
+    else launch<bf16, 2, 2, 2, 2, true, true, OUT>(g, used, s);
   }
-  if (large(2 * F, D, 256)) launch<4, 2, 2, 4, true, true, OUT>(g, used, s);
-  else launch<2, 2, 2, 2, true, true, OUT>(g, used, s);
   if (splits > 1) {
     hipLaunchKernelGGL(splits_kernel, dim3(flat_grid(2 * F * D)), dim3(256), 0, s, ptr<const float>(slabs), g.slab, used,
                        2 * F * D, ptr<void>(dw), dw_bf);

@@ -43,15 +43,15 @@ def _bf(t) -> bool:
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
-    """The matrix [rows, cols] as the kernels read it: bf16 rows start on 16 bytes and end on a multiple of 8 elements
-    (a copy with zeros behind each row where they do not)."""
+    """The matrix [rows, cols] as the kernels read it: rows start on 16 bytes and end on a multiple of 8 elements (a copy
+    with zeros behind each row where they do not)."""
     rows, cols = t.shape
-    if t.dtype != torch.bfloat16 or rows == 0 or (cols % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-                                                  and t.stride(0) >= cols):
+    if rows == 0 or (cols % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+                     and t.stride(0) >= cols):
         return t
     out = torch.empty(rows, -(-cols // 8) * 8, device=t.device, dtype=t.dtype)
     with device_guard(t):
-        load_native().gated_pad(t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0), True, rows, cols,
+        load_native().gated_pad(t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0), _bf(t), rows, cols,
                                 torch.cuda.current_stream(t.device).cuda_stream)
     return out
 
@@ -95,10 +95,11 @@ class _GatedLinear(torch.autograd.Function):
         else:
             nat = load_native()
             dh2 = rows_of(dh, Fo).to(x2.dtype)
-            half = -(-Fo // 8) * 8 if _bf(x2) else Fo
+            dh2 = _operand(dh2) if _bf(x2) else dh2
+            half = -(-Fo // 8) * 8
             dgu = mk(M, 2 * half, dt=x2.dtype)
-            part = mk(nat.gated_bias_workspace(_bf(x2), M, Fo), dt=torch.float32) if need_b else None
-            slabs = mk(nat.gated_weight_workspace(_bf(x2), M, D, Fo), dt=torch.float32) if need_w else None
+            part = mk(nat.gated_bias_workspace(M, Fo), dt=torch.float32) if need_b else None
+            slabs = mk(nat.gated_weight_workspace(M, D, Fo), dt=torch.float32) if need_w else None
             with device_guard(x2):
                 s = torch.cuda.current_stream(x2.device).cuda_stream
                 nat.gated_backward_pair(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _bf(x2), _p(bias), _bf(bias),
