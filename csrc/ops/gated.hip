@@ -24,7 +24,7 @@ typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
@@ -81,17 +81,19 @@ struct Bias {
 __device__ __forceinline__ constexpr int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Tiles.  out = sum_k A(r, k) B(c, k) on BM x BN tiles, K in steps of 128 bytes (64 bf16, 32 fp32), both operands copied
-// straight from memory into LDS (buffer loads to LDS, 16 bytes a lane) one step ahead of the products.
+// Tiles.  out = sum_k A(r, k) B(c, k) on BM x BN tiles, K in steps of 128 bytes (64 bf16, 32 fp32).  A step's operands
+// are loaded into registers two steps before they are stored to LDS and three before the products take them: the
+// products alone (2048 cycles a step on a 256 x 256 tile) hide less than the latency of loads that miss the L2.
 //
 //   row operand (k contiguous)    LDS [R][128 B], 16-byte chunk c of row r in slot c ^ ((r >> 1) & 7): the 16 rows of a
 //                                 fragment read cover all 64 banks once
 //   column operand (r contiguous) LDS [k][R]; bf16: chunk c of row k in slot c ^ 4 (k & 3), so the four rows of a
 //                                 transposing read (ds_read_b64_tr_b16) fall on four different quarters of the banks;
 //                                 fp32: slot c ^ 8 ((k >> 2) & 1), so the two halves of a wave read different banks
-// The copy to LDS writes lane l's 16 bytes at 16 l, so the slots are permuted on the address side.  Rows and chunks
-// outside the matrices get an offset past the buffer descriptor's end: the load returns zeros.  Operands are 16-byte
-// aligned with rows of a multiple of 8 elements (the caller pads others), so a chunk is inside or outside as a whole.
+// Lane l of a wave copy holds the 16 bytes of slot l of its 1 KB of LDS: the slots are permuted on the address side.  Rows
+// and chunks outside the matrices get an offset past the buffer descriptor's end: the load returns zeros.  Operands are
+// 16-byte aligned with rows of a multiple of 8 elements (the caller pads others), so a chunk is inside or outside as a
+// whole.
 
 constexpr unsigned kOut = 0x80000000u;   // past every descriptor (2^31 - 1 bytes)
 
@@ -121,36 +123,34 @@ struct Copy {
   static constexpr int PER = R / 8 / WAVES;   // 1 KB wave copies per wave and step
   static constexpr int CH = Elem<T>::CHUNK;
   static_assert(R % (8 * WAVES) == 0 && (!COL || R == 128 || R == 256), "tile");
+  static constexpr int CPR = COL ? R / CH : 8;   // chunks per stored row
   unsigned off[PER];
-  int kk[PER];      // k (row operand: of the chunk's first element; column operand: of the row) inside a step
   long step;        // elements per step
+  static __device__ __forceinline__ int row_of(int i, int wave, int lane) { return (i * WAVES + wave) * 64 / CPR + lane / CPR; }
+  static __device__ __forceinline__ int chunk_of(int r, int lane) {
+    return (lane % CPR) ^ (!COL ? (r >> 1) & 7 : CH == 8 ? (r & 3) << 2 : ((r >> 2) & 1) << 3);
+  }
   // r0: first row (column) of the tile, rows: their count in the matrix, ld: elements between stored rows
   __device__ __forceinline__ void init(long r0, long rows, long ld, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int q = i * WAVES + wave;
-      if (!COL) {
-        const int r = 8 * q + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-        off[i] = r0 + r < rows ? (unsigned)(r * ld * sizeof(T) + 16 * c) : kOut;
-        kk[i] = CH * c;
-      } else {
-        constexpr int CPR = R / CH;   // chunks per stored row
-        const int k = q * 64 / CPR + lane / CPR;
-        const int c = (lane % CPR) ^ (CH == 8 ? (k & 3) << 2 : ((k >> 2) & 1) << 3);
-        off[i] = r0 + CH * c < rows ? (unsigned)(k * ld * sizeof(T) + 16 * c) : kOut;
-        kk[i] = k;
-      }
+      const int r = row_of(i, wave, lane), c = chunk_of(r, lane);
+      off[i] = (COL ? r0 + CH * c : r0 + r) < rows ? (unsigned)(r * ld * sizeof(T) + 16 * c) : kOut;
     }
     step = COL ? Elem<T>::STEP * ld : Elem<T>::STEP;
   }
-  // base: the tile's first element at this step, left: k that remain (>= a step: all)
-  __device__ __forceinline__ void load(const T* base, long left, T* img, int wave) const {
+  // Piece i.  base: the tile's first element at this step, left: k that remain (>= a step: all)
+  __device__ __forceinline__ u32x4 load(int i, const T* base, long left, int wave, int lane) const {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, 0x7fffffff, 0x00027000);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const unsigned o = left >= Elem<T>::STEP || kk[i] < left ? off[i] : kOut;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_char*)((char*)img + 1024 * (i * WAVES + wave)), 16, o, 0, 0, 0);
+    unsigned o = off[i];
+    if (left < Elem<T>::STEP) {
+      const int r = row_of(i, wave, lane);
+      o = (COL ? r : CH * chunk_of(r, lane)) < left ? o : kOut;
     }
+    return __builtin_amdgcn_raw_buffer_load_b128(rs, o, 0, 0);
+  }
+  static __device__ __forceinline__ void store(int i, const u32x4& reg, T* img, int wave, int lane) {
+    *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(img) + 1024 * (i * WAVES + wave) + 16 * lane) = reg;
   }
 };
 
@@ -277,24 +277,103 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
   ca.init(m0, g.M, g.lda, wave, lane);
   cb.init(n0, g.N, g.ldb, wave, lane);
   const long a0 = (ACOL ? m0 + k0 * g.lda : m0 * g.lda + k0) + up * g.half, b0 = BCOL ? n0 + k0 * g.ldb : n0 * g.ldb + k0;
-  auto load = [&](int t, int buf) {
-    const int seg = t >= steps ? 1 : 0, st = t - seg * steps;
-    const long left = kend - k0 - (long)E::STEP * st;
-    ca.load(reinterpret_cast<const T*>(g.a[PAIR ? 0 : seg]) + a0 + st * ca.step, left, ia + buf * ASZ, wave);
-    const long bo = b0 + st * cb.step;
-    if (PAIR) {
-      cb.load(reinterpret_cast<const T*>(g.b[0]) + bo, left, ib + buf * BSZ, wave);
-      cb.load(reinterpret_cast<const T*>(g.b[1]) + bo, left, ib + buf * BSZ + BH * E::STEP, wave);
-    } else {
-      cb.load(reinterpret_cast<const T*>(g.b[seg]) + bo, left, ib + buf * BSZ, wave);
-    }
+  // Two sets of registers: a step's operands wait in set t & 1.
+  constexpr int PA = Copy<T, BM, WAVES, ACOL>::PER, PB = Copy<T, BH, WAVES, BCOL>::PER, NB = PAIR ? 2 : 1;
+  u32x4 ra[2][PA], rb[2][NB][PB];
+  auto left_of = [&](int t) { return t < total ? kend - k0 - (long)E::STEP * (t - (t >= steps ? steps : 0)) : 0; };
+  auto load_a = [&](int t, int set, int i) {   // t >= total: zeros
+    const int seg = t >= steps && g.segs > 1 ? 1 : 0;
+    ra[set][i] = ca.load(i, reinterpret_cast<const T*>(g.a[PAIR ? 0 : seg]) + a0 + (t - seg * steps) * ca.step, left_of(t),
+                         wave, lane);
+  };
+  auto load_b = [&](int t, int set, int i) {
+    const int seg = t >= steps && g.segs > 1 ? 1 : 0, q = i / PB;
+    rb[set][q][i % PB] = cb.load(i % PB, reinterpret_cast<const T*>(g.b[PAIR ? q : seg]) + b0 + (t - seg * steps) * cb.step,
+                                 left_of(t), wave, lane);
+  };
+  auto store_a = [&](int set, int buf, int i) { ca.store(i, ra[set][i], ia + buf * ASZ, wave, lane); };
+  auto store_b = [&](int set, int buf, int i) {
+    cb.store(i % PB, rb[set][i / PB][i % PB], ib + buf * BSZ + i / PB * BH * E::STEP, wave, lane);
   };
   Frags<T, BM, ACOL, RM> fa_at;
   Frags<T, BH, BCOL, SH> fb_at;
   fa_at.init(ia, 32 * wm * RM, lane);
   fb_at.init(ib, 32 * wn * SH, lane);
 
-  // bf16 backward: the tile of dh waits in registers behind the products
+  f32x16 acc[RM][RN];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < RN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  // A quarter of a step: the products of fragments that are there, each fragment of A replaced by the next quarter's
+  // right behind its last product, B's read into a second set; the stores and loads of a later step's operands in
+  // between.  So nothing waits for LDS but the barrier of each step, which stands before its last quarter, when the
+  // next step's operands are stored.  (The order is pinned: the scheduler would gather the reads and wait for them.)
+  typename E::frag fa[RM], fb[2][RN];
+  auto read_a = [&](int i, int s, int buf) { fa[i] = fa_at.read(i, s, buf * ASZ); };
+  auto read_b = [&](int s, int buf) {
+#pragma unroll
+    for (int j = 0; j < RN; ++j) fb[s & 1][j] = fb_at.read(j % SH, s, buf * BSZ + (j / SH) * BH * E::STEP);
+  };
+  auto quarter = [&](int t, int buf, int s) {
+    if (s == 3) lds_barrier();
+    const int ns = (s + 1) & 3, nbuf = s == 3 ? buf ^ 1 : buf;
+    read_b(ns, nbuf);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+#pragma unroll
+      for (int j = 0; j < RN; ++j)
+        acc[i][j] = SWAP ? E::mma(fb[s & 1][j], fa[i], acc[i][j]) : E::mma(fa[i], fb[s & 1][j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      read_a(i, ns, nbuf);
+      if (s == 1) {
+#pragma unroll
+        for (int q = i * PA / RM; q < (i + 1) * PA / RM; ++q) {
+          store_a(buf ^ 1, buf ^ 1, q);
+          load_a(t + 3, buf ^ 1, q);
+        }
+      }
+      if (s == 2) {
+#pragma unroll
+        for (int q = i * NB * PB / RM; q < (i + 1) * NB * PB / RM; ++q) {
+          store_b(buf ^ 1, buf ^ 1, q);
+          load_b(t + 3, buf ^ 1, q);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < 3; ++t) {
+    if (t == 2) {
+#pragma unroll
+      for (int q = 0; q < PA; ++q) store_a(0, 0, q);
+#pragma unroll
+      for (int q = 0; q < NB * PB; ++q) store_b(0, 0, q);
+    }
+#pragma unroll
+    for (int q = 0; q < PA; ++q) load_a(t, t & 1, q);
+#pragma unroll
+    for (int q = 0; q < NB * PB; ++q) load_b(t, t & 1, q);
+  }
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < RM; ++i) read_a(i, 0, 0);
+  read_b(0, 0);
+  // Steps go in pairs without a branch between them (an odd count ends with a step of zeros): across a branch the
+  // compiler waits for every load that either side may have sent.
+  for (int t = 0; t < total; t += 2) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) quarter(t, 0, s);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) quarter(t + 1, 1, s);
+  }
+
+  // bf16 backward: the tile of dh passes through registers
   constexpr int DPT = EPI == BWD && SWAP ? BM * BH / 8 / NT : 1;
   s16x8 dh[DPT];
   if constexpr (EPI == BWD && SWAP) {
@@ -305,58 +384,6 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
       if (m0 + row < g.M && n0 + c < g.N)
         dh[q] = *reinterpret_cast<const s16x8*>(reinterpret_cast<const short*>(g.dh) + (m0 + row) * g.lddh + n0 + c);
     }
-  }
-
-  f32x16 acc[RM][RN];
-#pragma unroll
-  for (int i = 0; i < RM; ++i)
-#pragma unroll
-    for (int j = 0; j < RN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
-  typename E::frag fa[2][RM], fb[2][RN];
-  auto read = [&](int s, int buf) {
-#pragma unroll
-    for (int i = 0; i < RM; ++i) fa[s & 1][i] = fa_at.read(i, s, buf * ASZ);
-#pragma unroll
-    for (int j = 0; j < RN; ++j) fb[s & 1][j] = fb_at.read(j % SH, s, buf * BSZ + (j / SH) * BH * E::STEP);
-  };
-  auto mul = [&](int s) {
-#pragma unroll
-    for (int i = 0; i < RM; ++i)
-#pragma unroll
-      for (int j = 0; j < RN; ++j)
-        acc[i][j] = SWAP ? E::mma(fb[s & 1][j], fa[s & 1][i], acc[i][j]) : E::mma(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
-  };
-  // The next step's copies have landed and every wave has taken its last fragments of this one: its images are free.
-  auto turn = [&] {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-  // Fragments are read one quarter ahead of the products, across the steps too, so the matrix cores have work while
-  // the waves meet at the barrier.
-  auto step = [&](int t, int buf) {
-#pragma unroll
-    for (int s = 0; s < 3; ++s) {
-      read(s + 1, buf);
-      mul(s);
-    }
-    if (t + 1 < total) {
-      turn();
-      if (t + 2 < total) load(t + 2, buf);
-      read(0, buf ^ 1);
-    }
-    mul(3);
-  };
-  load(0, 0);
-  turn();
-  if (total > 1) load(1, 1);
-  read(0, 0);
-  for (int t = 0; t < total; t += 2) {
-    step(t, 0);
-    if (t + 1 < total) step(t + 1, 1);
   }
 
   // ---- epilogue
