@@ -8,6 +8,8 @@
 // bf16 operands run on v_mfma_f32_32x32x16_bf16, fp32 on v_mfma_f32_32x32x2_f32.
 #include <hip/hip_bf16.h>
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 #include <pybind11/pybind11.h>
 
 #include "../common.h"
@@ -47,16 +49,18 @@ __device__ __forceinline__ float normal_cdf(float g, float& e) {
   return g < 0.f ? tail : 1.f - tail;
 }
 
-__device__ __forceinline__ float act_fwd(int act, float g) {
+template <int ACT>
+__device__ __forceinline__ float act_fwd(float g) {
   float e;
-  if (act == GELU) return g * normal_cdf(g, e);
+  if (ACT == GELU) return g * normal_cdf(g, e);
   const float s = sigmoid(g);
-  return act == SILU ? g * s : s;
+  return ACT == SILU ? g * s : s;
 }
 
 // a = act(g), d = act'(g)
-__device__ __forceinline__ void act_both(int act, float g, float& a, float& d) {
-  if (act == GELU) {
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float& a, float& d) {
+  if (ACT == GELU) {
     float e;
     const float phi = normal_cdf(g, e);
     a = g * phi;
@@ -64,8 +68,8 @@ __device__ __forceinline__ void act_both(int act, float g, float& a, float& d) {
     return;
   }
   const float s = sigmoid(g);
-  a = act == SILU ? g * s : s;
-  d = act == SILU ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
+  a = ACT == SILU ? g * s : s;
+  d = ACT == SILU ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
 }
 
 struct Bias {
@@ -140,7 +144,7 @@ struct Copy {
     step = COL ? Elem<T>::STEP * ld : Elem<T>::STEP;
   }
   // Piece i.  base: the tile's first element at this step, left: k that remain (>= a step: all)
-  __device__ __forceinline__ u32x4 load(int i, const T* base, long left, int wave, int lane) const {
+  __device__ __forceinline__ u32x4 load(int i, const T* base, int left, int wave, int lane) const {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, 0x7fffffff, 0x00027000);
     unsigned o = off[i];
     if (left < Elem<T>::STEP) {
@@ -200,7 +204,7 @@ struct TileArgs {
   int segs;
   long M, N, K;       // rows, columns (pair: F) and K of a segment
   int tm, tn;         // tiles
-  long kchunk;        // K of a split (whole steps; one segment only), K otherwise
+  int chunk;          // steps of a split (blockIdx.y)
   Bias bias;
   const void* dh;
   long lddh;
@@ -242,6 +246,15 @@ __device__ __forceinline__ float half_wave_sum(float v) {
   return v;
 }
 
+// finish(activation) with the activation as a constant: a branch per element would keep the elements' exponentials and
+// reciprocals from overlapping.
+template <bool PAIR, class F>
+__host__ __device__ __forceinline__ void by_act(int act, F&& finish) {
+  if (PAIR && act == GELU) finish(std::integral_constant<int, GELU>{});
+  else if (PAIR && act == SIGMOID) finish(std::integral_constant<int, SIGMOID>{});
+  else finish(std::integral_constant<int, SILU>{});
+}
+
 // What leaves a tile: FWD h, BWD dgu (and the bias gradient's partial sums), OUT the product in T, SUM in fp32 (split
 // partial results, gradients of fp32 masters).
 enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3 };
@@ -249,7 +262,7 @@ enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3 };
 // bf16 tiles swap the operands of the matrix instruction, so that a lane holds four neighbouring columns of one row and
 // stages them in LDS with one 8-byte write; fp32 results leave from the accumulators as 128-byte row pieces.
 template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
   typedef Elem<T> E;
   constexpr int WAVES = WM * WN, NT = 64 * WAVES, BM = 32 * RM * WM, BN = 32 * RN * WN;
   constexpr bool PAIR = EPI == FWD || EPI == BWD, SWAP = E::CHUNK == 8 && EPI != SUM;
@@ -258,39 +271,72 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
   constexpr int ASZ = BM * E::STEP, BSZ = BN * E::STEP, OPS = 2 * (ASZ + BSZ) * (int)sizeof(T);
   constexpr int OC = EPI == FWD ? BH : BN, OLD = OC + 8;   // output columns of the tile, staged row stride
   constexpr int STG = SWAP ? BM * OLD * 2 : 0;
-  __shared__ __attribute__((aligned(1024))) char smem[OPS > STG ? OPS : STG];
+  constexpr int USE = OPS > STG ? OPS : STG, BIAS = PAIR ? 2 * BH * 4 : 0;
+  static_assert(!PAIR || 2 * BH <= NT, "a bias element per thread");
+  __shared__ __attribute__((aligned(1024))) char smem[USE + BIAS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  int pm, pn;
-  tile_of(blockIdx.x, g.tm, g.tn, pm, pn);
-  const int up = !PAIR && g.tmh && pm >= g.tmh;   // dW: rows of the up half
-  const int part_row = pm * WM + wm;
-  if (up) pm -= g.tmh;
-  const long m0 = (long)pm * BM, n0 = (long)pn * BH;
-  const long k0 = (long)blockIdx.y * g.kchunk, kend = k0 + g.kchunk < g.K ? k0 + g.kchunk : g.K;
-  const int steps = (int)((kend - k0 + E::STEP - 1) / E::STEP), total = steps * g.segs;
+  // steps of a segment; first and number of this split's, over all segments
+  const int steps = (int)((g.K + E::STEP - 1) / E::STEP), t0 = blockIdx.y * g.chunk;
+  const int total = min(g.chunk, steps * g.segs - t0);
 
   // two images of each operand: A0 A1 | B0 B1
   T *const ia = reinterpret_cast<T*>(smem), *const ib = ia + 2 * ASZ;
-  Copy<T, BM, WAVES, ACOL> ca;
-  Copy<T, BH, WAVES, BCOL> cb;
-  ca.init(m0, g.M, g.lda, wave, lane);
-  cb.init(n0, g.N, g.ldb, wave, lane);
-  const long a0 = (ACOL ? m0 + k0 * g.lda : m0 * g.lda + k0) + up * g.half, b0 = BCOL ? n0 + k0 * g.ldb : n0 * g.ldb + k0;
+  float* const sbias = reinterpret_cast<float*>(smem + USE);   // bg, bu of the tile's columns
   // Two sets of registers: a step's operands wait in set t & 1.
   constexpr int PA = Copy<T, BM, WAVES, ACOL>::PER, PB = Copy<T, BH, WAVES, BCOL>::PER, NB = PAIR ? 2 : 1;
   u32x4 ra[2][PA], rb[2][NB][PB];
-  auto left_of = [&](int t) { return t < total ? kend - k0 - (long)E::STEP * (t - (t >= steps ? steps : 0)) : 0; };
-  auto load_a = [&](int t, int set, int i) {   // t >= total: zeros
-    const int seg = t >= steps && g.segs > 1 ? 1 : 0;
-    ra[set][i] = ca.load(i, reinterpret_cast<const T*>(g.a[PAIR ? 0 : seg]) + a0 + (t - seg * steps) * ca.step, left_of(t),
-                         wave, lane);
+  Copy<T, BM, WAVES, ACOL> ca;
+  Copy<T, BH, WAVES, BCOL> cb;
+  int pm, pn;
+  tile_of(blockIdx.x, g.tm, g.tn, pm, pn);
+  const int up = !PAIR && g.tmh && pm >= g.tmh, part_row = pm * WM + wm;   // up: rows of dW's up half
+  if (up) pm -= g.tmh;
+  const long m0 = (long)pm * BM, n0 = (long)pn * BH;
+  const long a0 = (ACOL ? m0 : m0 * g.lda) + up * g.half, b0 = BCOL ? n0 : n0 * g.ldb;
+  ca.init(m0, g.M, g.lda, wave, lane);
+  cb.init(n0, g.N, g.ldb, wave, lane);
+  // Where the next loads of A and of B are: steps of both segments in order, then zeros.
+  struct Cursor {
+    const T* p;
+    int left, count;   // k that remain in the segment, steps of the split
   };
-  auto load_b = [&](int t, int set, int i) {
-    const int seg = t >= steps && g.segs > 1 ? 1 : 0, q = i / PB;
-    rb[set][q][i % PB] = cb.load(i % PB, reinterpret_cast<const T*>(g.b[PAIR ? q : seg]) + b0 + (t - seg * steps) * cb.step,
-                                 left_of(t), wave, lane);
+  auto start = [&](const void* const* base, long at, long step, bool two) {
+    const int seg = two && t0 >= steps ? 1 : 0, st = t0 - seg * steps;
+    return Cursor{reinterpret_cast<const T*>(base[seg]) + at + st * step, (int)g.K - E::STEP * st, total};
   };
+  auto advance = [&](Cursor& c, const void* const* base, long at, long step, bool two) {
+    c.p += step;
+    c.left -= E::STEP;
+    if (two && c.left <= 0) {
+      c.p = reinterpret_cast<const T*>(base[1]) + at;
+      c.left = (int)g.K;
+    }
+    if (--c.count <= 0) c.left = 0;
+  };
+  const bool two = !PAIR && g.segs > 1;
+  const long wu = PAIR ? reinterpret_cast<const T*>(g.b[1]) - reinterpret_cast<const T*>(g.b[0]) : 0;   // up rows
+  Cursor at_a = start(g.a, a0, ca.step, two), at_b = start(g.b, b0, cb.step, two);
+  auto load_a = [&](int set, int i) {
+    ra[set][i] = ca.load(i, at_a.p, at_a.left, wave, lane);
+    if (i == PA - 1) advance(at_a, g.a, a0, ca.step, two);
+  };
+  auto load_b = [&](int set, int i) {
+    rb[set][i / PB][i % PB] = cb.load(i % PB, at_b.p + i / PB * wu, at_b.left, wave, lane);
+    if (i == NB * PB - 1) advance(at_b, g.b, b0, cb.step, two);
+  };
+  auto load = [&](int set) {
+#pragma unroll
+    for (int q = 0; q < PA; ++q) load_a(set, q);
+#pragma unroll
+    for (int q = 0; q < NB * PB; ++q) load_b(set, q);
+  };
+  load(0);
+  load(1);
+  if (PAIR && tid < 2 * BH) {
+    const long n = n0 + tid % BH;
+    sbias[tid] = n < g.N ? g.bias.at(tid < BH ? n : g.N + n) : 0.f;
+  }
   auto store_a = [&](int set, int buf, int i) { ca.store(i, ra[set][i], ia + buf * ASZ, wave, lane); };
   auto store_b = [&](int set, int buf, int i) {
     cb.store(i % PB, rb[set][i / PB][i % PB], ib + buf * BSZ + i / PB * BH * E::STEP, wave, lane);
@@ -301,13 +347,6 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
   fb_at.init(ib, 32 * wn * SH, lane);
 
   f32x16 acc[RM][RN];
-#pragma unroll
-  for (int i = 0; i < RM; ++i)
-#pragma unroll
-    for (int j = 0; j < RN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
   // A quarter of a step: the products of fragments that are there, each fragment of A replaced by the next quarter's
   // right behind its last product, B's read into a second set; the stores and loads of a later step's operands in
   // between.  So nothing waits for LDS but the barrier of each step, which stands before its last quarter, when the
@@ -318,7 +357,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
 #pragma unroll
     for (int j = 0; j < RN; ++j) fb[s & 1][j] = fb_at.read(j % SH, s, buf * BSZ + (j / SH) * BH * E::STEP);
   };
-  auto quarter = [&](int t, int buf, int s) {
+  auto quarter = [&](int buf, int s) {
     if (s == 3) lds_barrier();
     const int ns = (s + 1) & 3, nbuf = s == 3 ? buf ^ 1 : buf;
     read_b(ns, nbuf);
@@ -334,32 +373,30 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
 #pragma unroll
         for (int q = i * PA / RM; q < (i + 1) * PA / RM; ++q) {
           store_a(buf ^ 1, buf ^ 1, q);
-          load_a(t + 3, buf ^ 1, q);
+          load_a(buf ^ 1, q);
         }
       }
       if (s == 2) {
 #pragma unroll
         for (int q = i * NB * PB / RM; q < (i + 1) * NB * PB / RM; ++q) {
           store_b(buf ^ 1, buf ^ 1, q);
-          load_b(t + 3, buf ^ 1, q);
+          load_b(buf ^ 1, q);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 #pragma unroll
-  for (int t = 0; t < 3; ++t) {
-    if (t == 2) {
+  for (int q = 0; q < PA; ++q) store_a(0, 0, q);
 #pragma unroll
-      for (int q = 0; q < PA; ++q) store_a(0, 0, q);
+  for (int q = 0; q < NB * PB; ++q) store_b(0, 0, q);
+  load(0);
 #pragma unroll
-      for (int q = 0; q < NB * PB; ++q) store_b(0, 0, q);
-    }
+  for (int i = 0; i < RM; ++i)
 #pragma unroll
-    for (int q = 0; q < PA; ++q) load_a(t, t & 1, q);
+    for (int j = 0; j < RN; ++j)
 #pragma unroll
-    for (int q = 0; q < NB * PB; ++q) load_b(t, t & 1, q);
-  }
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
   lds_barrier();
 #pragma unroll
   for (int i = 0; i < RM; ++i) read_a(i, 0, 0);
@@ -368,11 +405,12 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
   // compiler waits for every load that either side may have sent.
   for (int t = 0; t < total; t += 2) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) quarter(t, 0, s);
+    for (int s = 0; s < 4; ++s) quarter(0, s);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) quarter(t + 1, 1, s);
+    for (int s = 0; s < 4; ++s) quarter(1, s);
   }
 
+  // ---- epilogue
   // bf16 backward: the tile of dh passes through registers
   constexpr int DPT = EPI == BWD && SWAP ? BM * BH / 8 / NT : 1;
   s16x8 dh[DPT];
@@ -385,18 +423,19 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
         dh[q] = *reinterpret_cast<const s16x8*>(reinterpret_cast<const short*>(g.dh) + (m0 + row) * g.lddh + n0 + c);
     }
   }
-
-  // ---- epilogue
   if constexpr (!SWAP) {
+    auto finish = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
     const int row0 = 32 * wm * RM + 4 * (lane >> 5);
     const long left = g.M - m0 - row0;
 #pragma unroll
     for (int j = 0; j < SH; ++j) {
-      const long n = n0 + 32 * (wn * SH + j) + (lane & 31);
+      const int col = 32 * (wn * SH + j) + (lane & 31);
+      const long n = n0 + col;
       const bool in = n < g.N;
       float* o = reinterpret_cast<float*>(g.out) + blockIdx.y * g.slab + (m0 + row0 + up * g.M) * g.ldo + n;
       const float* dv = EPI == BWD ? reinterpret_cast<const float*>(g.dh) + (m0 + row0) * g.lddh + n : nullptr;
-      const float bg = PAIR && in ? g.bias.at(n) : 0.f, bu = PAIR && in ? g.bias.at(g.N + n) : 0.f;
+      const float bg = PAIR ? sbias[col] : 0.f, bu = PAIR ? sbias[BH + col] : 0.f;
       float sg = 0.f, su = 0.f;
 #pragma unroll
       for (int i = 0; i < RM; ++i)
@@ -406,7 +445,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
           if (in && row < left) {
             if constexpr (EPI == BWD) {
               float a, d;
-              act_both(g.act, acc[i][j][r] + bg, a, d);
+              act_both<ACT>(acc[i][j][r] + bg, a, d);
               const float u = acc[i][j + SH][r] + bu;
               const float dg = *dv * u * d, du = *dv * a;
               o[0] = dg;
@@ -414,7 +453,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
               sg += dg;
               su += du;
             } else if constexpr (EPI == FWD) {
-              *o = act_fwd(g.act, acc[i][j][r] + bg) * (acc[i][j + SH][r] + bu);
+              *o = act_fwd<ACT>(acc[i][j][r] + bg) * (acc[i][j + SH][r] + bu);
             } else {
               *o = acc[i][j][r];
             }
@@ -433,7 +472,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
         }
       }
     }
-    return;
+    };
+    by_act<PAIR>(g.act, finish);
   } else {
     short* stage = reinterpret_cast<short*>(smem);
     lds_barrier();   // the operand images are free
@@ -445,19 +485,18 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
       }
       lds_barrier();
     }
+    auto finish = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
 #pragma unroll
     for (int j = 0; j < SH; ++j) {
 #pragma unroll
       for (int rg = 0; rg < 4; ++rg) {
         const int col = 32 * (wn * SH + j) + 8 * rg + 4 * (lane >> 5);   // this lane's four columns
-        float bg[4], bu[4], sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
+        f32x4 bg, bu;
+        float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
         if (PAIR) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const long n = n0 + col + e;
-            bg[e] = n < g.N ? g.bias.at(n) : 0.f;
-            bu[e] = n < g.N ? g.bias.at(g.N + n) : 0.f;
-          }
+          bg = *reinterpret_cast<const f32x4*>(sbias + col);
+          bu = *reinterpret_cast<const f32x4*>(sbias + BH + col);
         }
 #pragma unroll
         for (int i = 0; i < RM; ++i) {
@@ -470,11 +509,11 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
             if constexpr (EPI == OUT) {
               v[e] = to_s(c);
             } else if constexpr (EPI == FWD) {
-              v[e] = to_s(act_fwd(g.act, c + bg[e]) * (acc[i][j + SH][4 * rg + e] + bu[e]));
+              v[e] = to_s(act_fwd<ACT>(c + bg[e]) * (acc[i][j + SH][4 * rg + e] + bu[e]));
             } else {
               // rows and columns outside have dh = 0
               float a, d;
-              act_both(g.act, c + bg[e], a, d);
+              act_both<ACT>(c + bg[e], a, d);
               const float x = to_f((short)w[e]);
               const float dg = x * (acc[i][j + SH][4 * rg + e] + bu[e]) * d, du = x * a;
               v[e] = to_s(dg);
@@ -499,6 +538,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
         }
       }
     }
+    };
+    by_act<PAIR>(g.act, finish);
     lds_barrier();
     // rows of the staged tile leave in 16-byte pieces; dgu rows are padded to whole pieces (with zeros), others may end
     // inside one or start off 16 bytes
@@ -521,6 +562,57 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(TileArgs g) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+
+// Few rows (M <= 16 MF): bound by reading the weights once.  A workgroup takes 16 columns of F and all rows; its 8 waves
+// take the k steps of 32 in turn (512 contiguous bytes of every weight row at a time), weights and rows straight from
+// memory into v_mfma_f32_16x16x32_bf16 fragments, and add their sums in LDS in order.  Rows and columns past the ends
+// repeat the last one: their results are not stored.
+template <int MF, int ACT>
+__global__ __launch_bounds__(512) void rows_kernel(const bf16* x, long ldx, const bf16* w, long ldw, Bias bias, bf16* h, int M,
+                                                   int K, long F) {
+  __shared__ f32x4 red[8][2][MF][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const long f0 = (long)blockIdx.x * 16, fr = f0 + r < F ? f0 + r : F - 1;
+  const bf16 *wg = w + fr * ldw, *wu = wg + F * ldw;
+  const bf16* xr[MF];
+  f32x4 g[MF], u[MF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+    xr[i] = x + (long)min(16 * i + r, M - 1) * ldx;
+    g[i] = u[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const bf16x8 zero = {};
+#pragma unroll 4
+  for (int k0 = 32 * wave; k0 < K; k0 += 256) {
+    const int k = k0 + 8 * q, kc = k < K ? k : 0;
+    const bf16x8 a = *reinterpret_cast<const bf16x8*>(wg + kc), b = *reinterpret_cast<const bf16x8*>(wu + kc);
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+      const bf16x8 c = *reinterpret_cast<const bf16x8*>(xr[i] + kc);
+      g[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k < K ? a : zero, k < K ? c : zero, g[i], 0, 0, 0);
+      u[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k < K ? b : zero, k < K ? c : zero, u[i], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+    red[wave][0][i][lane] = g[i];
+    red[wave][1][i][lane] = u[i];
+  }
+  __syncthreads();
+  if (wave >= MF) return;
+  const int m = 16 * wave + r;   // this lane: row m, columns f0 + 4 q ..
+  const long f = f0 + 4 * q;
+  f32x4 sg = red[0][0][wave][lane], su = red[0][1][wave][lane];
+#pragma unroll
+  for (int z = 1; z < 8; ++z) {
+    sg += red[z][0][wave][lane];
+    su += red[z][1][wave][lane];
+  }
+  if (m >= M) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (f + e < F) h[m * F + f + e] = __float2bfloat16(act_fwd<ACT>(sg[e] + bias.at(f + e)) * (su[e] + bias.at(F + f + e)));
+}
 
 // dst [rows][ldd]: the rows of src, zeros behind them.
 template <class T>
@@ -591,7 +683,9 @@ static void launch(TileArgs g, int splits, hipStream_t s) {
   if (g.tmh) g.tmh = (int)tm;
   g.tm = (int)(g.tmh ? 2 * tm : tm);
   g.tn = (int)tn;
-  hipLaunchKernelGGL((tile_kernel<T, RM, RN, WM, WN, ACOL, BCOL, EPI>), dim3((unsigned)(g.tm * g.tn), splits),
+  const int all = (int)(tiles(g.K, Elem<T>::STEP) * g.segs);
+  g.chunk = (int)tiles(all, splits);
+  hipLaunchKernelGGL((tile_kernel<T, RM, RN, WM, WN, ACOL, BCOL, EPI>), dim3((unsigned)(g.tm * g.tn), (unsigned)tiles(all, g.chunk)),
                      dim3(64 * WM * WN), 0, s, g);
   check_launch();
 }
@@ -601,6 +695,9 @@ static bool large(long M, long N, long bn) { return tiles(M, 256) * tiles(N, bn)
 static int pair_rows(long M, long F) { return large(M, F, 128) ? 256 : 128; }
 // Partial rows of the bias gradient: two wave rows a tile.
 static long part_rows(long M, long F) { return 2 * tiles(M, pair_rows(M, F)); }
+
+// Most rows of the few-rows kernel.
+constexpr long kRows = 32;
 
 template <class T, int EPI>
 static void pair(const TileArgs& g, hipStream_t s) {
@@ -622,7 +719,7 @@ static TileArgs pair_args(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, 
   g.segs = 1;
   g.M = M;
   g.N = F;
-  g.K = g.kchunk = up8(D);   // rows are padded with zeros
+  g.K = up8(D);   // rows are padded with zeros
   g.bias = Bias{ptr<const void>(bias), bias_bf};
   g.act = act;
   return g;
@@ -633,6 +730,19 @@ void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bia
   TileArgs g = pair_args(x, ldx, w, ldw, bf, bias, bias_bf, M, D, F, act);
   g.out = ptr<void>(h);
   g.ldo = F;
+  if (bf && M <= kRows) {
+    by_act<true>(act, [&](auto a) {
+      constexpr int ACT = decltype(a)::value;
+      auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, dim3((unsigned)tiles(F, 16)), dim3(512), 0, stream_of(stream), ptr<const bf16>(x), ldx,
+                           ptr<const bf16>(w), ldw, g.bias, ptr<bf16>(h), (int)M, (int)g.K, F);
+      };
+      if (M <= 16) go(rows_kernel<1, ACT>);
+      else go(rows_kernel<2, ACT>);
+    });
+    check_launch();
+    return;
+  }
   if (bf) pair<bf16, FWD>(g, stream_of(stream));
   else pair<float, FWD>(g, stream_of(stream));
 }
@@ -673,13 +783,39 @@ void backward_pair(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr
   }
 }
 
-void backward_x(uintptr_t dgu, uintptr_t w, long ldw, int bf, uintptr_t dx, int dx_bf, long M, long D, long F,
+// Splits of a product's K (t tiles of 128 x 128, `outputs` results): n splits divide the time of a tile's steps (0.7 us
+// each, of 64) by n and cost n fp32 results written and read again (4 TB/s): the n where the two are equal, two workgroups
+// per CU and at least 4 steps each.  dX of 256 / 2560 rows of 256 x 1024: 22.5 / 22.8 us unsplit, 10.8 / 17 us split;
+// of 25,600 rows 40 us unsplit, 58 us in two.
+static int k_splits(long t, long K, long outputs) {
+  const double n = std::sqrt((double)K / 64 * 0.7e-6 / ((double)outputs * 8 / 4e12));
+  return (int)std::max<long>(1, std::min<long>({(long)(n + 0.5), (2L * cu_count() + t - 1) / t, K / 256, 64}));
+}
+
+static int x_splits(long M, long D, long F) {
+  return large(M, D, 256) ? 1 : k_splits(tiles(M, 128) * tiles(D, 128), 2 * F, M * D);
+}
+long x_workspace(long M, long D, long F) {
+  const int n = x_splits(M, D, F);
+  return n > 1 ? n * M * D : 0;
+}
+
+static void add_splits(uintptr_t slabs, const TileArgs& g, int bf, int splits, long n, uintptr_t out, int out_bf, hipStream_t s) {
+  const long all = tiles(g.K, bf ? 64 : 32) * g.segs;
+  hipLaunchKernelGGL(splits_kernel, dim3(flat_grid(n)), dim3(256), 0, s, ptr<const float>(slabs), n,
+                     (int)tiles(all, tiles(all, splits)), n, ptr<void>(out), out_bf);
+  check_launch();
+}
+
+void backward_x(uintptr_t dgu, uintptr_t w, long ldw, int bf, uintptr_t dx, int dx_bf, uintptr_t slabs, long M, long D, long F,
                 uintptr_t stream) {
   check_sizes(M, D, F, 0);
   const hipStream_t s = stream_of(stream);
   check_operand(dgu, 2 * up8(F));
   check_operand(w, ldw);
-  const int es = bf ? 2 : 4;
+  const int es = bf ? 2 : 4, splits = x_splits(M, D, F);
+  GSC_CHECK(splits == 1 || slabs, "gated_linear: the input gradient needs a workspace");
+  GSC_CHECK(bf || !dx_bf, "gated_linear: fp32 operands give fp32 gradients");
   TileArgs g{};
   g.a[0] = ptr<const void>(dgu);
   g.a[1] = ptr<const void>(dgu + up8(F) * es);
@@ -690,28 +826,26 @@ void backward_x(uintptr_t dgu, uintptr_t w, long ldw, int bf, uintptr_t dx, int 
   g.segs = 2;
   g.M = M;
   g.N = D;
-  g.K = g.kchunk = F;
-  g.out = ptr<void>(dx);
+  g.K = F;
+  g.out = ptr<void>(splits > 1 ? slabs : dx);
   g.ldo = D;
-  const bool big = large(M, D, 256);
-  GSC_CHECK(bf || !dx_bf, "gated_linear: fp32 operands give fp32 gradients");
+  g.slab = M * D;
+  const bool big = large(M, D, 256), sum = splits > 1 || !dx_bf;
   if (!bf) {
-    if (big) launch<float, 4, 2, 2, 4, false, true, SUM>(g, 1, s);
-    else launch<float, 2, 2, 2, 2, false, true, SUM>(g, 1, s);
-  } else if (dx_bf) {
-    if (big) launch<bf16, 4, 2, 2, 4, false, true, OUT>(g, 1, s);
-    else launch<bf16, 2, 2, 2, 2, false, true, OUT>(g, 1, s);
+    if (big) launch<float, 4, 2, 2, 4, false, true, SUM>(g, splits, s);
+    else launch<float, 2, 2, 2, 2, false, true, SUM>(g, splits, s);
+  } else if (sum) {
+    if (big) launch<bf16, 4, 2, 2, 4, false, true, SUM>(g, splits, s);
+    else launch<bf16, 2, 2, 2, 2, false, true, SUM>(g, splits, s);
   } else {
-    if (big) launch<bf16, 4, 2, 2, 4, false, true, SUM>(g, 1, s);
-    else launch<bf16, 2, 2, 2, 2, false, true, SUM>(g, 1, s);
+    if (big) launch<bf16, 4, 2, 2, 4, false, true, OUT>(g, splits, s);
+    else launch<bf16, 2, 2, 2, 2, false, true, OUT>(g, splits, s);
   }
+  if (splits > 1) add_splits(slabs, g, bf, splits, M * D, dx, dx_bf, s);
 }
 
-// Splits of dW's reduction over the rows: enough workgroups for two per CU, at least 512 rows each.
 static int w_splits(long M, long D, long F) {
-  if (large(2 * F, D, 256)) return 1;
-  const long t = 2 * tiles(F, 128) * tiles(D, 128);
-  return (int)std::max<long>(1, std::min<long>({(2L * cu_count() + t - 1) / t, M / 512, 64}));
+  return large(2 * F, D, 256) ? 1 : k_splits(2 * tiles(F, 128) * tiles(D, 128), M, 2 * F * D);
 }
 
 long w_workspace(long M, long D, long F) {
@@ -737,29 +871,23 @@ void backward_w(uintptr_t dgu, uintptr_t x, long ldx, int bf, uintptr_t dw, int 
   g.M = F;
   g.N = D;
   g.K = M;
-  g.kchunk = tiles(tiles(M, splits), 64) * 64;
   g.half = up8(F);
   g.tmh = 1;
   g.ldo = D;
   g.slab = 2 * F * D;
   g.out = ptr<void>(splits > 1 ? slabs : dw);
-  const int used = (int)tiles(M, g.kchunk);
   const bool big = large(2 * F, D, 256), sum = splits > 1 || !dw_bf;
   if (!bf) {
-    if (big) launch<float, 4, 2, 2, 4, true, true, SUM>(g, used, s);
-    else launch<float, 2, 2, 2, 2, true, true, SUM>(g, used, s);
+    if (big) launch<float, 4, 2, 2, 4, true, true, SUM>(g, splits, s);
+    else launch<float, 2, 2, 2, 2, true, true, SUM>(g, splits, s);
   } else if (sum) {
-    if (big) launch<bf16, 4, 2, 2, 4, true, true, SUM>(g, used, s);
-    else launch<bf16, 2, 2, 2, 2, true, true, SUM>(g, used, s);
+    if (big) launch<bf16, 4, 2, 2, 4, true, true, SUM>(g, splits, s);
+    else launch<bf16, 2, 2, 2, 2, true, true, SUM>(g, splits, s);
   } else {
-    if (big) launch<bf16, 4, 2, 2, 4, true, true, OUT>(g, used, s);
-    else launch<bf16, 2, 2, 2, 2, true, true, OUT>(g, used, s);
+    if (big) launch<bf16, 4, 2, 2, 4, true, true, OUT>(g, splits, s);
+    else launch<bf16, 2, 2, 2, 2, true, true, OUT>(g, splits, s);
   }
-  if (splits > 1) {
-    hipLaunchKernelGGL(splits_kernel, dim3(flat_grid(2 * F * D)), dim3(256), 0, s, ptr<const float>(slabs), g.slab, used,
-                       2 * F * D, ptr<void>(dw), dw_bf);
-    check_launch();
-  }
+  if (splits > 1) add_splits(slabs, g, bf, splits, 2 * F * D, dw, dw_bf, s);
 }
 
 }  // namespace gated
@@ -768,6 +896,7 @@ void register_gated(py::module_& m) {
   m.def("gated_forward", &gated::forward, "h = act(x Wg^T + bg) * (x Wu^T + bu)");
   m.def("gated_pad", &gated::pad, "rows copied to a padded row length, zeros behind them");
   m.def("gated_bias_workspace", &gated::bias_workspace, "fp32 elements of the bias gradient's partial sums");
+  m.def("gated_input_workspace", &gated::x_workspace, "fp32 elements of the input gradient's partial results");
   m.def("gated_weight_workspace", &gated::w_workspace, "fp32 elements of the weight gradient's partial results");
   m.def("gated_backward_pair", &gated::backward_pair, "dgu = [dh u act'(g) | dh act(g)] and the bias gradient");
   m.def("gated_backward_x", &gated::backward_x, "dx = dgu W");

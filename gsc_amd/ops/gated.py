@@ -99,16 +99,17 @@ class _GatedLinear(torch.autograd.Function):
             half = -(-Fo // 8) * 8
             dgu = mk(M, 2 * half, dt=x2.dtype)
             part = mk(nat.gated_bias_workspace(M, Fo), dt=torch.float32) if need_b else None
-            slabs = mk(nat.gated_weight_workspace(M, D, Fo), dt=torch.float32) if need_w else None
             with device_guard(x2):
                 s = torch.cuda.current_stream(x2.device).cuda_stream
                 nat.gated_backward_pair(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _bf(x2), _p(bias), _bf(bias),
                                         dh2.data_ptr(), dh2.stride(0), dgu.data_ptr(), _p(part), _p(db), _bf(db), M, D, Fo,
                                         ctx.act, s)
                 if need_x:
-                    nat.gated_backward_x(dgu.data_ptr(), w.data_ptr(), w.stride(0), _bf(x2), dx.data_ptr(), _bf(dx), M, D,
-                                         Fo, s)
+                    xs = mk(nat.gated_input_workspace(M, D, Fo), dt=torch.float32)
+                    nat.gated_backward_x(dgu.data_ptr(), w.data_ptr(), w.stride(0), _bf(x2), dx.data_ptr(), _bf(dx),
+                                         xs.data_ptr(), M, D, Fo, s)
                 if need_w:
+                    slabs = mk(nat.gated_weight_workspace(M, D, Fo), dt=torch.float32)
                     nat.gated_backward_w(dgu.data_ptr(), x2.data_ptr(), x2.stride(0), _bf(x2), dw.data_ptr(), _bf(dw),
                                          slabs.data_ptr(), M, D, Fo, s)
         return dx.view(shape) if need_x else None, dw, db, None, None, None
