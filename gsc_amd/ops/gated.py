@@ -16,11 +16,10 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from gsc_amd.native import load as load_native
+from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, rows_of
 from .linear import shadow
-from .norm import _TYPES, check_cuda, device_guard, note_leaves, rows_of
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
 
@@ -34,14 +33,6 @@ def gated_linear_reference(x: torch.Tensor, weight: torch.Tensor, bias: Optional
     return (a * u).to(x.dtype)
 
 
-def _p(t) -> int:
-    return t.data_ptr() if t is not None else 0
-
-
-def _bf(t) -> bool:
-    return t is not None and t.dtype == torch.bfloat16
-
-
 def _operand(t: torch.Tensor) -> torch.Tensor:
     """The matrix [rows, cols] as the kernels read it: rows start on 16 bytes and end on a multiple of 8 elements (a copy
     with zeros behind each row where they do not)."""
@@ -50,9 +41,7 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
                      and t.stride(0) >= cols):
         return t
     out = torch.empty(rows, -(-cols // 8) * 8, device=t.device, dtype=t.dtype)
-    with device_guard(t):
-        load_native().gated_pad(t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0), _bf(t), rows, cols,
-                                torch.cuda.current_stream(t.device).cuda_stream)
+    launch(load_native().gated_pad, t, t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0), is_bf16(t), rows, cols)
     return out
 
 
@@ -61,9 +50,8 @@ def _forward(x2, w, bias, act, D):
     Fo = w.shape[0] // 2
     h = torch.empty(M, Fo, device=x2.device, dtype=x2.dtype)
     if M > 0:
-        with device_guard(x2):
-            load_native().gated_forward(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _bf(x2), _p(bias), _bf(bias),
-                                        h.data_ptr(), M, D, Fo, act, torch.cuda.current_stream(x2.device).cuda_stream)
+        launch(load_native().gated_forward, x2, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), is_bf16(x2), ptr(bias),
+               is_bf16(bias), h.data_ptr(), M, D, Fo, act)
     return h
 
 
@@ -78,7 +66,7 @@ class _GatedLinear(torch.autograd.Function):
         return h.view(*x.shape[:-1], h.shape[1])
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, dh):
         x2, w, bias = ctx.saved_tensors
         shape, x_dtype = ctx.x
@@ -95,23 +83,21 @@ class _GatedLinear(torch.autograd.Function):
         else:
             nat = load_native()
             dh2 = rows_of(dh, Fo).to(x2.dtype)
-            dh2 = _operand(dh2) if _bf(x2) else dh2
+            dh2 = _operand(dh2) if is_bf16(x2) else dh2
             half = -(-Fo // 8) * 8
             dgu = mk(M, 2 * half, dt=x2.dtype)
             part = mk(nat.gated_bias_workspace(M, Fo), dt=torch.float32) if need_b else None
-            with device_guard(x2):
-                s = torch.cuda.current_stream(x2.device).cuda_stream
-                nat.gated_backward_pair(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _bf(x2), _p(bias), _bf(bias),
-                                        dh2.data_ptr(), dh2.stride(0), dgu.data_ptr(), _p(part), _p(db), _bf(db), M, D, Fo,
-                                        ctx.act, s)
-                if need_x:
-                    xs = mk(nat.gated_input_workspace(M, D, Fo), dt=torch.float32)
-                    nat.gated_backward_x(dgu.data_ptr(), w.data_ptr(), w.stride(0), _bf(x2), dx.data_ptr(), _bf(dx),
-                                         xs.data_ptr(), M, D, Fo, s)
-                if need_w:
-                    slabs = mk(nat.gated_weight_workspace(M, D, Fo), dt=torch.float32)
-                    nat.gated_backward_w(dgu.data_ptr(), x2.data_ptr(), x2.stride(0), _bf(x2), dw.data_ptr(), _bf(dw),
-                                         slabs.data_ptr(), M, D, Fo, s)
+            launch(nat.gated_backward_pair, x2, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), is_bf16(x2), ptr(bias),
+                   is_bf16(bias), dh2.data_ptr(), dh2.stride(0), dgu.data_ptr(), ptr(part), ptr(db), is_bf16(db), M, D, Fo,
+                   ctx.act)
+            if need_x:
+                slabs = mk(nat.gated_input_workspace(M, D, Fo), dt=torch.float32)
+                launch(nat.gated_backward_x, x2, dgu.data_ptr(), w.data_ptr(), w.stride(0), is_bf16(x2), dx.data_ptr(),
+                       is_bf16(dx), slabs.data_ptr(), M, D, Fo)
+            if need_w:
+                slabs = mk(nat.gated_weight_workspace(M, D, Fo), dt=torch.float32)
+                launch(nat.gated_backward_w, x2, dgu.data_ptr(), x2.data_ptr(), x2.stride(0), is_bf16(x2), dw.data_ptr(),
+                       is_bf16(dw), slabs.data_ptr(), M, D, Fo)
         return dx.view(shape) if need_x else None, dw, db, None, None, None
 
 
@@ -132,10 +118,8 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         raise ValueError(f"gated_linear: w16 must be bfloat16 {tuple(weight.shape)}, got {w16.dtype} {tuple(w16.shape)}")
     if not x.is_cuda:
         return gated_linear_reference(x, weight, bias, activation)
-    for k, t in (("x", x), ("weight", weight), ("bias", bias)):
-        if t is not None and t.dtype not in _TYPES:
-            raise TypeError(f"gated_linear: {k} must be bfloat16 or float32 on the GPU, got {t.dtype}")
-    check_cuda("gated_linear", x, weight=weight, bias=bias, w16=w16)
+    check_types("gated_linear", x=x, weight=weight, bias=bias)
+    check_device("gated_linear", x, weight=weight, bias=bias, w16=w16)
     dtype = x.dtype
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")

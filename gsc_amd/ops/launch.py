@@ -1,0 +1,79 @@
+"""What the wrappers of the feed-forward operators share: argument checks, row views, launches, autograd rules."""
+from __future__ import annotations
+
+import functools
+
+import torch
+from torch.autograd.function import once_differentiable as _once_differentiable
+
+TYPES = (torch.bfloat16, torch.float32)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def launch(fn, t: torch.Tensor, *args) -> None:
+    """``fn(*args, stream)`` on the device of ``t`` (made current if it is not) and its current stream."""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            fn(*args, _raw_stream(dev))
+
+
+def ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def is_bf16(t) -> bool:
+    return t is not None and t.dtype is torch.bfloat16
+
+
+def rows_of(t: torch.Tensor, C: int) -> torch.Tensor:
+    """[rows, C] view of ``t`` with contiguous rows (a copy only where its strides allow no such view)."""
+    t = t if t.dim() == 2 else t.reshape(-1, C)
+    return t if C == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def check_device(name: str, x: torch.Tensor, **others) -> None:
+    for k, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name}: {k} is on {t.device}, x on {x.device}")
+
+
+def check_types(name: str, **tensors) -> None:
+    for k, t in tensors.items():
+        if t is not None and t.dtype not in TYPES:
+            raise TypeError(f"{name}: {k} must be bfloat16 or float32 on the GPU, got {t.dtype}")
+
+
+def differentiable_once(backward):
+    """``once_differentiable`` at no cost to a plain backward pass (its wrapper is used under ``create_graph`` only)."""
+    checked = _once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
+_STREAM = "gsc_amd.stream"
+
+
+def note_leaves(name: str, out: torch.Tensor, *inputs) -> torch.Tensor:
+    """Refuses to capture an op on a leaf whose gradient node lives in a graph made on another stream.
+
+    Autograd keeps one gradient node per leaf for as long as any graph holds it, bound to the stream it was made on.  A
+    backward pass captured later would make that stream, outside the capture, wait for the captured one, which ends the
+    process when the capture ends.  ``inputs``: the Function's tensor arguments in order (None: absent)."""
+    nodes = None
+    for i, t in enumerate([t for t in inputs if t is not None]):
+        if not (t.requires_grad and t.is_leaf):
+            continue
+        if nodes is None:
+            nodes, stream = out.grad_fn.next_functions, _raw_stream(out.get_device())
+        if (nodes[i][0].metadata.setdefault(_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing()):
+            raise RuntimeError(f"{name}: a graph of the same leaf tensor {tuple(t.shape)}, made on another stream, is still "
+                               "alive; a captured backward pass cannot share its gradient node (drop the outputs of "
+                               "earlier calls before the capture, or capture with leaves of its own)")
+    return out

@@ -14,10 +14,9 @@ from typing import Optional, Union
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from gsc_amd.native import load as load_native
-from .norm import _TYPES, check_cuda, device_guard, note_leaves
+from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr
 
 _M32 = np.uint64(0xFFFFFFFF)
 
@@ -64,13 +63,10 @@ def dropout_reference(x: torch.Tensor, p: float, seed: int, offset: int = 0,
 
 def _launch(x, res, p, seed, offset, at, keep_at):
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    if x.numel() > 0:
-        with device_guard(x):
-            load_native().dropout(x.data_ptr(), res.data_ptr() if res is not None else 0, y.data_ptr(),
-                                  x.dtype == torch.bfloat16, x.numel(), seed, offset,
-                                  at.data_ptr() if at is not None else 0,
-                                  keep_at.data_ptr() if keep_at is not None else 0, p,
-                                  torch.cuda.current_stream(x.device).cuda_stream)
+    n = x.numel()
+    if n > 0:
+        launch(load_native().dropout, x, x.data_ptr(), ptr(res), y.data_ptr(), is_bf16(x), n, seed, offset, ptr(at),
+               ptr(keep_at), p)
     return y
 
 
@@ -84,7 +80,7 @@ class _Dropout(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, dy):
         (used,) = ctx.saved_tensors
         dx = _launch(dy.contiguous(), None, *ctx.args, used, None) if ctx.needs_input_grad[0] else None
@@ -115,9 +111,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
                          f"{residual.dtype}")
     if not x.is_cuda:
         return dropout_reference(x, p, seed, offset, residual)
-    if x.dtype not in _TYPES:
-        raise TypeError(f"dropout: x must be bfloat16 or float32 on the GPU, got {x.dtype}")
-    check_cuda("dropout", x, residual=residual)
+    check_types("dropout", x=x)
+    check_device("dropout", x, residual=residual)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return note_leaves("dropout", _Dropout.apply(x, residual, float(p), int(seed), int(offset), at), x, residual)
     return _launch(x.contiguous(), residual.contiguous() if residual is not None else None, float(p), int(seed),
