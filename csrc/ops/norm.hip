@@ -391,13 +391,12 @@ static int vec_of(uintptr_t x, long ldx, uintptr_t y, long ldy, uintptr_t w, uin
   return (x | y | w | b) % 16 == 0 && ldx % v == 0 && ldy % v == 0 && C % v == 0 ? v : 1;
 }
 
-// Partial rows of the backward: workgroups, each over rows / workgroups rows (at most 1,024 and 4 MB of partial sums, at
-// least 64).
+// Partial rows of the backward: workgroups, each over rows / workgroups rows (at most 1,024, and 8 MB of partial sums or 512).
 static int parts_of(long M, long C, int vec) {
   const Shape sh = shape_of(C, vec);
   if (!sh.g) return (int)std::max<long>(1, std::min<long>(256, M / 16));
   const long wg = sh.g > 256 ? 1 : 256 / sh.g;
-  return (int)std::max<long>(1, std::min<long>({(M + wg - 1) / wg, 1024, std::max<long>(256, (1L << 20) / (2 * C))}));
+  return (int)std::max<long>(1, std::min<long>({(M + wg - 1) / wg, 1024, std::max<long>(512, (1L << 21) / (2 * C))}));
 }
 
 // f(lanes, pieces) with both as constants.

@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, rows_of
+from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
 from .linear import shadow
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
@@ -62,42 +62,42 @@ class _GatedLinear(torch.autograd.Function):
         x2, w = _operand(rows_of(x, D).to(dtype)), _operand(w)
         h = _forward(x2, w, bias, act, D)
         ctx.save_for_backward(x2, w, bias)
-        ctx.act, ctx.x, ctx.w_dtype = act, (x.shape, x.dtype), weight.dtype
-        return h.view(*x.shape[:-1], h.shape[1])
+        nat, M, Fo = load_native(), x2.shape[0], h.shape[1]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        ctx.nat, ctx.act, ctx.dev, ctx.x, ctx.w_dtype = nat, act, x.get_device(), (x.shape, x.dtype), weight.dtype
+        ctx.sizes = (M, D, Fo)
+        ctx.space = (nat.gated_input_workspace(M, D, Fo) if M and need_x else 0,
+                     nat.gated_weight_workspace(M, D, Fo) if M and need_w else 0,
+                     nat.gated_bias_workspace(M, Fo) if M and need_b else 0)
+        return h.view(*x.shape[:-1], Fo)
 
     @staticmethod
     @differentiable_once
     def backward(ctx, dh):
         x2, w, bias = ctx.saved_tensors
-        shape, x_dtype = ctx.x
-        M, D, Fo = x2.shape[0], shape[-1], w.shape[0] // 2
+        (shape, x_dtype), (M, D, Fo), space = ctx.x, ctx.sizes, ctx.space
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        mk = lambda *s, dt: torch.empty(*s, device=x2.device, dtype=dt)
-        dx = mk(M, D, dt=x_dtype) if need_x else None
-        dw = mk(2 * Fo, D, dt=ctx.w_dtype) if need_w else None
-        db = mk(2 * Fo, dt=bias.dtype) if need_b else None
+        dev, bf = x2.device, is_bf16(x2)
+        dx = torch.empty(M, D, device=dev, dtype=x_dtype) if need_x else None
+        dw = torch.empty(2 * Fo, D, device=dev, dtype=ctx.w_dtype) if need_w else None
+        db = torch.empty(2 * Fo, device=dev, dtype=bias.dtype) if need_b else None
         if M == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
         else:
-            nat = load_native()
+            nat, s = ctx.nat, raw_stream(ctx.dev)
             dh2 = rows_of(dh, Fo).to(x2.dtype)
-            dh2 = _operand(dh2) if is_bf16(x2) else dh2
-            half = -(-Fo // 8) * 8
-            dgu = mk(M, 2 * half, dt=x2.dtype)
-            part = mk(nat.gated_bias_workspace(M, Fo), dt=torch.float32) if need_b else None
-            launch(nat.gated_backward_pair, x2, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), is_bf16(x2), ptr(bias),
-                   is_bf16(bias), dh2.data_ptr(), dh2.stride(0), dgu.data_ptr(), ptr(part), ptr(db), is_bf16(db), M, D, Fo,
-                   ctx.act)
+            dh2 = _operand(dh2) if bf else dh2
+            dgu = torch.empty(M, 2 * (-(-Fo // 8) * 8), device=dev, dtype=x2.dtype)
+            xp, wp, gp, xl, wl = x2.data_ptr(), w.data_ptr(), dgu.data_ptr(), x2.stride(0), w.stride(0)
+            work = [torch.empty(n, device=dev) if n else None for n in space]
+            nat.gated_backward_pair(xp, xl, wp, wl, bf, ptr(bias), is_bf16(bias), dh2.data_ptr(), dh2.stride(0), gp,
+                                    ptr(work[2]), ptr(db), is_bf16(db), M, D, Fo, ctx.act, s)
             if need_x:
-                slabs = mk(nat.gated_input_workspace(M, D, Fo), dt=torch.float32)
-                launch(nat.gated_backward_x, x2, dgu.data_ptr(), w.data_ptr(), w.stride(0), is_bf16(x2), dx.data_ptr(),
-                       is_bf16(dx), slabs.data_ptr(), M, D, Fo)
+                nat.gated_backward_x(gp, wp, wl, bf, dx.data_ptr(), is_bf16(dx), ptr(work[0]), M, D, Fo, s)
             if need_w:
-                slabs = mk(nat.gated_weight_workspace(M, D, Fo), dt=torch.float32)
-                launch(nat.gated_backward_w, x2, dgu.data_ptr(), x2.data_ptr(), x2.stride(0), is_bf16(x2), dw.data_ptr(),
-                       is_bf16(dw), slabs.data_ptr(), M, D, Fo)
+                nat.gated_backward_w(gp, xp, xl, bf, dw.data_ptr(), is_bf16(dw), ptr(work[1]), M, D, Fo, s)
         return dx.view(shape) if need_x else None, dw, db, None, None, None
 
 

@@ -7,17 +7,17 @@ import torch
 from torch.autograd.function import once_differentiable as _once_differentiable
 
 TYPES = (torch.bfloat16, torch.float32)
-_raw_stream = torch._C._cuda_getCurrentRawStream
+raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def launch(fn, t: torch.Tensor, *args) -> None:
     """``fn(*args, stream)`` on the device of ``t`` (made current if it is not) and its current stream."""
     dev = t.get_device()
     if dev == torch.cuda.current_device():
-        fn(*args, _raw_stream(dev))
+        fn(*args, raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            fn(*args, _raw_stream(dev))
+            fn(*args, raw_stream(dev))
 
 
 def ptr(t) -> int:
@@ -47,12 +47,16 @@ def check_types(name: str, **tensors) -> None:
 
 
 def differentiable_once(backward):
-    """``once_differentiable`` at no cost to a plain backward pass (its wrapper is used under ``create_graph`` only)."""
+    """``once_differentiable`` at little cost to a plain backward pass: its wrapper is used under ``create_graph`` only.
+
+    (What a backward pass does in Python runs on autograd's own thread, two to three times slower than the same lines of
+    the forward pass, so the Functions prepare their launches in ``forward``.  Autograd makes the device of the forward
+    call current there.)"""
     checked = _once_differentiable(backward)
 
     @functools.wraps(backward)
-    def run(ctx, *grads):
-        return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+    def run(ctx, grad, enabled=torch.is_grad_enabled):
+        return checked(ctx, grad) if enabled() else backward(ctx, grad)
 
     return run
 
@@ -71,7 +75,7 @@ def note_leaves(name: str, out: torch.Tensor, *inputs) -> torch.Tensor:
         if not (t.requires_grad and t.is_leaf):
             continue
         if nodes is None:
-            nodes, stream = out.grad_fn.next_functions, _raw_stream(out.get_device())
+            nodes, stream = out.grad_fn.next_functions, raw_stream(out.get_device())
         if (nodes[i][0].metadata.setdefault(_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing()):
             raise RuntimeError(f"{name}: a graph of the same leaf tensor {tuple(t.shape)}, made on another stream, is still "
                                "alive; a captured backward pass cannot share its gradient node (drop the outputs of "

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, rows_of
+from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
 
 
 def layer_norm_reference(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -47,33 +47,35 @@ class _LayerNorm(torch.autograd.Function):
         x2 = rows_of(x, x.shape[-1])
         y, st = _forward(x2, weight, bias, eps, True)
         ctx.save_for_backward(x2, weight, st)
-        ctx.shape, ctx.bias = x.shape, None if bias is None else bias.dtype
+        M, C = x2.shape
+        nat, need, bf = load_native(), ctx.needs_input_grad, is_bf16(x2)
+        ctx.sizes, ctx.dev, ctx.run = (M, C, x.shape), x.get_device(), nat.layer_norm_backward
+        ctx.types = (weight.dtype if need[1] else None, bias.dtype if need[2] else None)
+        ctx.flags = (bf, is_bf16(weight))
+        ctx.part = nat.layer_norm_workspace(M, C, bf) if M and (need[1] or need[2]) else 0
         return y.view(x.shape)
 
     @staticmethod
     @differentiable_once
     def backward(ctx, dy):
         x2, weight, st = ctx.saved_tensors
-        M, C = x2.shape
-        need, dev = ctx.needs_input_grad, x2.device
-        dx = torch.empty(M, C, device=dev, dtype=x2.dtype) if need[0] else None
-        dw = torch.empty(C, device=dev, dtype=weight.dtype) if need[1] else None
-        db = torch.empty(C, device=dev, dtype=ctx.bias) if need[2] else None
+        (M, C, shape), (bf, w_bf), (wt, bt) = ctx.sizes, ctx.flags, ctx.types
+        dev = x2.device
+        dx = torch.empty(M, C, device=dev, dtype=x2.dtype) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(C, device=dev, dtype=wt) if wt is not None else None
+        db = torch.empty(C, device=dev, dtype=bt) if bt is not None else None
         if M == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
-        elif need[0] or need[1] or need[2]:
-            nat = load_native()
+        else:
             dy2 = rows_of(dy, C)
-            part = None
-            if need[1] or need[2]:
-                part = torch.empty(nat.layer_norm_workspace(M, C, is_bf16(x2)), device=dev, dtype=torch.float32)
+            part = torch.empty(ctx.part, device=dev) if ctx.part else None
             s0 = st.data_ptr()
-            launch(nat.layer_norm_backward, x2, x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), is_bf16(x2),
-                   ptr(weight), is_bf16(weight), s0, s0 + 4 * M, ptr(dx), ptr(dw), is_bf16(dw), ptr(db), is_bf16(db),
-                   ptr(part), M, C)
-        return dx.view(ctx.shape) if dx is not None else None, dw, db, None
+            ctx.run(x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), bf, ptr(weight), w_bf, s0, s0 + 4 * M,
+                    ptr(dx), ptr(dw), wt is torch.bfloat16, ptr(db), bt is torch.bfloat16, ptr(part), M, C,
+                    raw_stream(ctx.dev))
+        return dx.view(shape) if dx is not None else None, dw, db, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,

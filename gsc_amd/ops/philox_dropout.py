@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr
+from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream
 
 _M32 = np.uint64(0xFFFFFFFF)
 
@@ -74,17 +74,22 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, offset, at):
         used = torch.empty(1, device=x.device, dtype=torch.int64) if at is not None else None
-        y = _launch(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed, offset, at, used)
-        ctx.save_for_backward(used)
-        ctx.args = (p, seed, offset)
-        return y
+        ctx.used = used   # the offset this call read
+        ctx.args = (is_bf16(x), x.numel(), seed, offset, ptr(used), 0, p)
+        ctx.run, ctx.dev = load_native().dropout, x.get_device()
+        return _launch(x.contiguous(), residual.contiguous() if residual is not None else None, p, seed, offset, at, used)
 
     @staticmethod
     @differentiable_once
     def backward(ctx, dy):
-        (used,) = ctx.saved_tensors
-        dx = _launch(dy.contiguous(), None, *ctx.args, used, None) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
+        need_x, need_res = ctx.needs_input_grad[:2]
+        dx = None
+        if need_x:
+            dy = dy.contiguous()
+            dx = torch.empty_like(dy)
+            if ctx.args[1]:
+                ctx.run(dy.data_ptr(), 0, dx.data_ptr(), *ctx.args, raw_stream(ctx.dev))
+        return dx, dy if need_res else None, None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tensor] = 0,
