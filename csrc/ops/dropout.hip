@@ -62,7 +62,37 @@ __device__ __forceinline__ uint32_t keep_bits(uint64_t seed, uint64_t group, uin
   return keep;
 }
 
-template <class T>
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+// The 8 elements of a group, 16-byte aligned.
+struct Eight {
+  float v[8];
+  __device__ __forceinline__ void load(const float* p) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+  }
+  __device__ __forceinline__ void load(const __hip_bfloat16* p) {
+    const s16x8 a = *reinterpret_cast<const s16x8*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __bfloat162float(__builtin_bit_cast(__hip_bfloat16, (short)a[e]));
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    reinterpret_cast<f32x4*>(p)[0] = f32x4{v[0], v[1], v[2], v[3]};
+    reinterpret_cast<f32x4*>(p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+  }
+  __device__ __forceinline__ void store(__hip_bfloat16* p) const {
+    s16x8 a;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = __builtin_bit_cast(short, __float2bfloat16(v[e]));
+    *reinterpret_cast<s16x8*>(p) = a;
+  }
+};
+
+// A thread takes whole groups.  The loads are sent before the generator runs (about 20 wide multiplies and 60 other
+// instructions a group), so its arithmetic hides behind them: the kernel runs at the rate of the memory.
+template <class T, bool ALIGNED>
 __global__ __launch_bounds__(256) void drop_kernel(const T* x, const T* res, T* y, long n, uint64_t seed, uint64_t offset,
                                                    const long long* offset_ptr, long long* offset_out, uint32_t thr,
                                                    float scale) {
@@ -70,12 +100,27 @@ __global__ __launch_bounds__(256) void drop_kernel(const T* x, const T* res, T* 
   if (offset_ptr) offset = (uint64_t)*offset_ptr & ~(1ull << 63);
   if (offset_out && first == 0) *offset_out = (long long)offset;
   for (long g = first; g < groups; g += (long)gridDim.x * 256) {
+    const long i0 = 8 * g;
+    const bool whole = ALIGNED && i0 + 8 <= n;
+    Eight a, b;
+    if (whole) {
+      a.load(x + i0);
+      if (res) b.load(res + i0);
+    }
     const uint32_t keep = keep_bits(seed, (uint64_t)g, offset, thr);
-    for (int j = 0; j < 8 && 8 * g + j < n; ++j) {
-      const long i = 8 * g + j;
-      float v = (keep >> j) & 1u ? to_f(x[i]) * scale : 0.f;
-      if (res) v += to_f(res[i]);
-      y[i] = from_f<T>(v);
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        a.v[j] = (keep >> j) & 1u ? a.v[j] * scale : 0.f;
+        if (res) a.v[j] += b.v[j];
+      }
+      a.store(y + i0);
+    } else {
+      for (int j = 0; j < 8 && i0 + j < n; ++j) {
+        float v = (keep >> j) & 1u ? to_f(x[i0 + j]) * scale : 0.f;
+        if (res) v += to_f(res[i0 + j]);
+        y[i0 + j] = from_f<T>(v);
+      }
     }
   }
 }
@@ -91,8 +136,12 @@ void run(uintptr_t x, uintptr_t res, uintptr_t y, int bf16, long n, uint64_t see
   const hipStream_t s = stream_of(stream);
   auto go = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL((drop_kernel<T>), dim3(grid), dim3(256), 0, s, ptr<const T>(x), ptr<const T>(res), ptr<T>(y), n,
-                       seed, offset, ptr<const long long>(offset_ptr), ptr<long long>(offset_out), thr, scale);
+    auto launch = [&](auto kern) {
+      hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, s, ptr<const T>(x), ptr<const T>(res), ptr<T>(y), n, seed, offset,
+                         ptr<const long long>(offset_ptr), ptr<long long>(offset_out), thr, scale);
+    };
+    if ((x | res | y) % 16 == 0) launch(drop_kernel<T, true>);
+    else launch(drop_kernel<T, false>);
   };
   if (bf16) go((__hip_bfloat16*)nullptr);
   else go((float*)nullptr);
