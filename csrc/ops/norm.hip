@@ -340,22 +340,21 @@ __global__ __launch_bounds__(256) void bwd_long_sums_kernel(const T* x, long ldx
   part[((long)blockIdx.y * 2 + 1) * C + c] = db;
 }
 
-// Sum of the partial rows: 16 columns x 16 row phases a workgroup, phases added in order.
-__global__ __launch_bounds__(256) void sums_kernel(const float* part, int rows, int C, void* dw, int dw_bf, void* db,
-                                                   int db_bf) {
-  __shared__ float red[16][17];
+// Sum of the partial rows: 16 columns x 64 row phases a workgroup, phases added in order.
+__global__ __launch_bounds__(1024) void sums_kernel(const float* part, int rows, int C, void* dw, int dw_bf, void* db,
+                                                    int db_bf) {
+  __shared__ float red[64][17];
   const int cl = threadIdx.x & 15, ph = threadIdx.x >> 4;
   const long k = (long)blockIdx.x * 16 + cl;   // column of [dw | db]
   float s = 0.f;
   if (k < 2L * C) {
 #pragma unroll 8
-    for (int z = ph; z < rows; z += 16) s += part[(long)z * 2 * C + k];
+    for (int z = ph; z < rows; z += 64) s += part[(long)z * 2 * C + k];
   }
   red[ph][cl] = s;
   __syncthreads();
   if (ph || k >= 2L * C) return;
-#pragma unroll
-  for (int q = 1; q < 16; ++q) s += red[q][cl];
+  for (int q = 1; q < 64; ++q) s += red[q][cl];
   const bool second = k >= C;
   void* out = second ? db : dw;
   if (!out) return;
@@ -366,23 +365,21 @@ __global__ __launch_bounds__(256) void sums_kernel(const float* part, int rows, 
 
 // ---- launches
 
-// Lanes per row and pieces per lane of a row of C elements in pieces of VEC: the fewest lanes that hold it in two pieces
-// each, up to a wave, then up to eight; then workgroups of 256 and 1,024 lanes.  g = 0: too long for registers.
+// Lanes per row and pieces per lane of a row of C elements in pieces of VEC: the fewest lanes that hold it in 16 elements
+// each (8 where an element is a piece) -- the backward pass keeps five values an element in registers, and with 32 of them
+// too few waves fit to cover the loads (16384 x 8192 bf16: 237 us with 256 lanes, 175 us with 512).
+// g = 0: too long for registers.
 struct Shape {
   int g, n;
 };
 static Shape shape_of(long C, int vec) {
   const long p = (C + vec - 1) / vec;   // pieces
-  const int most = vec == 8 ? 4 : 8;    // 32 elements a lane
   for (int g : {8, 16, 32, 64})
     if (p <= g) return {g, 1};
-  for (int n : {2, 4, 8})
-    if (n <= most && p <= 64L * n) return {64, n};
-  for (int n : {2, 4, 8})
-    if (n <= most && p <= 256L * n) return {256, n};
-  const int wide = vec == 8 ? 2 : vec == 4 ? 4 : 8;   // 16 elements a lane (8 where an element is a piece)
-  for (int n : {2, 4, 8})
-    if (n <= wide && p <= 1024L * n) return {1024, n};
+  const int most = vec == 8 ? 2 : vec == 4 ? 4 : 8;
+  for (int g : {64, 256, 512, 1024})
+    for (int n : {1, 2, 4, 8})
+      if (n <= most && (g == 256 || 2 * n >= most) && p <= (long)g * n) return {g, n};
   return {0, 0};
 }
 
@@ -407,13 +404,13 @@ static void by_shape(Shape sh, F&& f) {
     f(std::integral_constant<int, G>{}, std::integral_constant<int, N>{});   \
     return;                                                                  \
   }
-  GSC_SHAPE(8, 1) GSC_SHAPE(16, 1) GSC_SHAPE(32, 1) GSC_SHAPE(64, 1) GSC_SHAPE(64, 2) GSC_SHAPE(64, 4)
-  GSC_SHAPE(256, 2) GSC_SHAPE(256, 4) GSC_SHAPE(1024, 2)
-  if constexpr (VEC != 8) {
-    GSC_SHAPE(64, 8) GSC_SHAPE(256, 8) GSC_SHAPE(1024, 4)
-  }
-  if constexpr (VEC == 1) {
-    GSC_SHAPE(1024, 8)
+  GSC_SHAPE(8, 1) GSC_SHAPE(16, 1) GSC_SHAPE(32, 1) GSC_SHAPE(64, 1)
+  if constexpr (VEC == 8) {
+    GSC_SHAPE(64, 2) GSC_SHAPE(256, 1) GSC_SHAPE(256, 2) GSC_SHAPE(512, 2) GSC_SHAPE(1024, 2)
+  } else if constexpr (VEC == 4) {
+    GSC_SHAPE(64, 2) GSC_SHAPE(64, 4) GSC_SHAPE(256, 2) GSC_SHAPE(256, 4) GSC_SHAPE(512, 4) GSC_SHAPE(1024, 4)
+  } else {
+    GSC_SHAPE(64, 4) GSC_SHAPE(64, 8) GSC_SHAPE(256, 4) GSC_SHAPE(256, 8) GSC_SHAPE(512, 8) GSC_SHAPE(1024, 8)
   }
 #undef GSC_SHAPE
   GSC_CHECK(false, "layer_norm: no kernel for this shape");
@@ -495,7 +492,7 @@ void backward(uintptr_t x, long ldx, uintptr_t dy, long lddy, int bf, uintptr_t 
   else if (vec == 4) run_bwd<float, 4>(x, ldx, dy, lddy, pw, mean, rstd, dx, p, M, (int)C, s);
   else run_bwd<float, 1>(x, ldx, dy, lddy, pw, mean, rstd, dx, p, M, (int)C, s);
   if (params) {
-    hipLaunchKernelGGL(sums_kernel, dim3((unsigned)((2 * C + 15) / 16)), dim3(256), 0, s, ptr<const float>(part),
+    hipLaunchKernelGGL(sums_kernel, dim3((unsigned)((2 * C + 15) / 16)), dim3(1024), 0, s, ptr<const float>(part),
                        parts_of(M, C, vec), (int)C, ptr<void>(dw), dw_bf, ptr<void>(db), db_bf);
     check_launch();
   }
