@@ -24,7 +24,9 @@ static uintptr_t create_cu_masked_stream(std::vector<int> cus) {
     mask[c / 32] |= 1u << (c % 32);
   }
   hipStream_t s = nullptr;
-  GSC_HIP_CHECK(hipExtStreamCreateWithCUMask(&s, (uint32_t)mask.size(), mask.data()));
+  const hipError_t e = hipExtStreamCreateWithCUMask(&s, (uint32_t)mask.size(), mask.data());
+  if (e != hipSuccess) (void)hipGetLastError();  // the caller may go on with another mask
+  GSC_HIP_CHECK(e);
   return reinterpret_cast<uintptr_t>(s);
 }
 

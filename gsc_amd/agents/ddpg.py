@@ -586,9 +586,15 @@ class BatchedTrainer:
                 self.sim_cus = k
                 small_env = (160 * 1024) // max(int(sim.ctx.lds_per_env), 1) >= 4
                 sim_list = self.sim_cu_list(n, k, spread_default=small_env)
+                try:
+                    handle = nat.create_cu_masked_stream(sim_list)
+                except RuntimeError:
+                    # some drivers refuse a spread mask of fewer than 8 bits per 32-bit block (it leaves XCDs without a
+                    # CU); contiguous bits are dealt to the XCDs in turn
+                    sim_list = list(range(k))
+                    handle = nat.create_cu_masked_stream(sim_list)
                 rest = [c for c in range(n) if c not in set(sim_list)]
-                self.sim_stream = torch.cuda.ExternalStream(nat.create_cu_masked_stream(sim_list),
-                                                            device=self.device)
+                self.sim_stream = torch.cuda.ExternalStream(handle, device=self.device)
                 # The learner stream is restricted to the complement, so no learner wave shares a SIMD
                 # with a simulator wave -- when the simulator is the critical path (small topologies whose
                 # envs pack three per CU: 103.6k vs 102.3k env-steps/s unmasked, 256 Abilene envs).  When
