@@ -19,6 +19,7 @@ act (actor forward) -> exploration + post-processing kernel -> simulator kernel 
 from __future__ import annotations
 
 import collections
+import contextlib
 import copy
 import ctypes
 import math
@@ -61,6 +62,11 @@ class DDPGLearner:
         torch.manual_seed(seed)
         self.actor = Actor(cfg, obs_dim, action_dim).to(self.device)
         self.critic = QNetwork(cfg, obs_dim, action_dim).to(self.device)
+        # dropout (a config option) is active only where a network's own loss is taken (_training); each network has its own
+        # masks, a function of the seed and the number of updates
+        for k, m in enumerate((self.actor, self.critic)):
+            m.mlp.seed_dropout(seed * 0x5851F42D4C957F2D + k + 1)
+            m.eval()
         self.target_actor = copy.deepcopy(self.actor)
         self.target_critic = copy.deepcopy(self.critic)
         if zero is None:
@@ -110,7 +116,9 @@ class DDPGLearner:
         self.compose_actor_critic = os.environ.get("GSC_COMPOSE", "1") != "0"
         # GPU: the update runs on hand-written kernels only (native_update.py); GSC_NATIVE_LEARNER=0
         # selects the autograd + PyTorch path (the CPU path, and the reference for the GPU tests)
+        # (networks with the optional hidden parts of gsc_amd/models/nets.py take that path too)
         self.native_ok = (self.device.type == "cuda" and self.amp and self.actor.graph_mode
+                          and self.actor.mlp.plain and self.critic.mlp.plain
                           and os.environ.get("GSC_NATIVE_LEARNER", "1") != "0")
         self._native = None
         self._topo_ready = False
@@ -122,6 +130,14 @@ class DDPGLearner:
             # must not keep cached casts alive across replays
             return torch.autocast(device_type=self.device.type, dtype=torch.bfloat16, cache_enabled=False)
         return torch.autocast(device_type=self.device.type, enabled=False)
+
+    @contextlib.contextmanager
+    def _training(self, net):
+        net.train()
+        try:
+            yield
+        finally:
+            net.eval()
 
     def refresh_shadows(self) -> None:
         """Re-derive the bf16 shadows after parameters were written outside the optimizer."""
@@ -170,8 +186,10 @@ class DDPGLearner:
     def _stage_critic(self, b: Batch) -> None:
         """TD target + critic loss -> critic gradients in ``critic_flat.grad``."""
         g, masks = self.graphs, self.masks
+        for net in (self.actor, self.critic):
+            net.mlp.advance_dropout()
         y = self._target(b)
-        with self._autocast():
+        with self._autocast(), self._training(self.critic):
             q = self.critic(b.obs, b.topo, g, masks, b.actions[:, :self.actor.action_dim]).float().view(-1)
             lq = F.mse_loss(q, y)
         grads = torch.autograd.grad(lq, self.critic_flat.params)
@@ -184,7 +202,7 @@ class DDPGLearner:
                 and not self.actor.squash and self.actor.graph_mode)
 
     def _stage_actor_fwd(self, b: Batch) -> None:
-        with self._autocast():
+        with self._autocast(), self._training(self.actor):
             if self._composed():
                 self._a = self.actor.hidden(b.obs, b.topo, self.graphs, self.masks)
             else:
@@ -351,6 +369,9 @@ class DDPGLearner:
         self.last = self._metrics_now()
 
     def _capture(self, b: Batch, inv_world: float, pre=None) -> None:
+        if not self.native_ok:   # an eager graph of the old leaves may be alive
+            self.critic_flat.renew_parameters()
+            self.actor_flat.renew_parameters()
         # thread-local capture: the RCCL watchdog thread keeps querying its events while we capture
         pool = torch.cuda.graph_pool_handle()
         stages, self._split = self._stages(b, inv_world)
@@ -428,6 +449,9 @@ class DDPGLearner:
         self.actor_opt.load_state_dict(opts["actor_opt"])
         self.critic_opt.load_state_dict(opts["critic_opt"])
         self.updates = int(sd.get("updates", 0))
+        for net in (self.actor, self.critic):   # the dropout masks go on where they were
+            if net.mlp.dropout:
+                net.mlp.drop_step.fill_(self.updates)
         if self._act_native is not None:  # weights written outside the optimizer
             self._act_native.rowtab_dirty = True
 

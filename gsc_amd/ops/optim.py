@@ -52,6 +52,19 @@ class FlatParams:
         self.grad = torch.zeros_like(self.flat)
         self.flat16 = None
 
+    def renew_parameters(self) -> None:
+        """New Parameter objects over the same storage in the module's places.
+
+        Autograd keeps a leaf's gradient node, and the stream it was made on, while any graph of the leaf lives; a graph
+        capture starts from leaves that no earlier graph can hold."""
+        for k, (name, p) in enumerate(zip(self.names, self.params)):
+            path, _, leaf = name.rpartition(".")
+            q = nn.Parameter(p.detach(), requires_grad=p.requires_grad)
+            if hasattr(p, "_bf16"):
+                q._bf16 = p._bf16
+            self.module.get_submodule(path)._parameters[leaf] = q
+            self.params[k] = q
+
     def enable_shadow(self) -> None:
         """Keep a bf16 copy of the parameters (``param._bf16`` views) for the bf16 GEMMs.
 
