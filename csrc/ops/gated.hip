@@ -2,8 +2,9 @@
 //
 //   weight [2F][D] = Wg over Wu, bias [2F] = bg, bu;  act: silu g s(g), gelu g Phi(g), sigmoid s(g)
 //   forward     both products of a tile in one kernel; bias, activation, product and rounding in its epilogue
-//   backward    g and u again (nothing but x is kept), dg = dh u act'(g), du = dh act(g) from the fp32 accumulators,
-//               rounded once to the operand type;  dx = dg Wg + du Wu,  dW = [dg | du]^T x,  db = column sums (fp32)
+//   backward    g and u from the fp32 accumulators again -- kept by the forward pass, or computed once more where that
+//               is cheaper (saves()) -- dg = dh u act'(g), du = dh act(g), rounded once to the operand type;
+//               dx = dg Wg + du Wu,  dW = [dg | du]^T x,  db = column sums (fp32)
 //
 // bf16 operands run on v_mfma_f32_32x32x16_bf16, fp32 on v_mfma_f32_32x32x2_f32.
 #include <hip/hip_bf16.h>
@@ -126,7 +127,7 @@ template <class T, int R, int WAVES, bool COL>
 struct Copy {
   static constexpr int PER = R / 8 / WAVES;   // 1 KB wave copies per wave and step
   static constexpr int CH = Elem<T>::CHUNK;
-  static_assert(R % (8 * WAVES) == 0 && (!COL || R == 128 || R == 256), "tile");
+  static_assert(R % (8 * WAVES) == 0 && (!COL || R >= (CH == 8 ? 128 : 64)), "tile");
   static constexpr int CPR = COL ? R / CH : 8;   // chunks per stored row
   unsigned off[PER];
   long step;        // elements per step
@@ -214,15 +215,17 @@ struct TileArgs {
   long slab;          // elements between the fp32 partial results of two splits
   int tmh;            // dW: tile rows of the gate half (the up half follows), 0 otherwise
   float* part;
+  float* saved;       // accumulators of the pair products, [tile][register quarter][thread][4]
   int act;
 };
 
-// Workgroups are dealt to the 8 XCDs in turn: each XCD takes a contiguous run of tiles, walked in strips of 8 tile
-// rows, so the operand panels its 32 CUs share stay in its own L2.
+// Workgroups are dealt to the 8 XCDs in turn: each XCD takes a contiguous run of tiles, walked in strips of 8 tile rows
+// (fewer where its run is short: about square), so the operand panels its CUs share stay in its own L2.
 __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& pm, int& pn) {
   const int total = tm * tn, per = total / 8, rem = total % 8, x = id & 7;
   const int t = x * per + (x < rem ? x : rem) + (id >> 3);
-  const int width = 8 * tn, g = t / width, first = g * 8, rows = tm - first < 8 ? tm - first : 8;
+  const int h = per >= 32 ? 8 : per >= 8 ? 4 : 2;
+  const int width = h * tn, g = t / width, first = g * h, rows = tm - first < h ? tm - first : h;
   pm = first + (t % width) % rows;
   pn = (t % width) / rows;
 }
@@ -261,14 +264,15 @@ enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3 };
 
 // bf16 tiles swap the operands of the matrix instruction, so that a lane holds four neighbouring columns of one row and
 // stages them in LDS with one 8-byte write; fp32 results leave from the accumulators as 128-byte row pieces.
-template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
+// KEPT (BWD): the products come from `saved`.
+template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT = false>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
   typedef Elem<T> E;
   constexpr int WAVES = WM * WN, NT = 64 * WAVES, BM = 32 * RM * WM, BN = 32 * RN * WN;
   constexpr bool PAIR = EPI == FWD || EPI == BWD, SWAP = E::CHUNK == 8 && EPI != SUM;
   constexpr int BH = PAIR ? BN / 2 : BN;            // columns of one product
   constexpr int SH = PAIR ? RN / 2 : RN;            // 32-column fragments of one product per wave
-  constexpr int ASZ = BM * E::STEP, BSZ = BN * E::STEP, OPS = 2 * (ASZ + BSZ) * (int)sizeof(T);
+  constexpr int ASZ = BM * E::STEP, BSZ = BN * E::STEP, OPS = KEPT ? 0 : 2 * (ASZ + BSZ) * (int)sizeof(T);
   constexpr int OC = EPI == FWD ? BH : BN, OLD = OC + 8;   // output columns of the tile, staged row stride
   constexpr int STG = SWAP ? BM * OLD * 2 : 0;
   constexpr int USE = OPS > STG ? OPS : STG, BIAS = PAIR ? 2 * BH * 4 : 0;
@@ -331,8 +335,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
 #pragma unroll
     for (int q = 0; q < NB * PB; ++q) load_b(set, q);
   };
-  load(0);
-  load(1);
+  if constexpr (!KEPT) {
+    load(0);
+    load(1);
+  }
   if (PAIR && tid < 2 * BH) {
     const long n = n0 + tid % BH;
     sbias[tid] = n < g.N ? g.bias.at(tid < BH ? n : g.N + n) : 0.f;
@@ -386,6 +392,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  if constexpr (!KEPT) {
 #pragma unroll
   for (int q = 0; q < PA; ++q) store_a(0, 0, q);
 #pragma unroll
@@ -409,8 +416,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) quarter(1, s);
   }
+  }
 
   // ---- epilogue
+  if constexpr (PAIR) {
+    f32x4* kept = reinterpret_cast<f32x4*>(g.saved) + ((long)pm * g.tn + pn) * (RM * RN * 4) * NT + tid;
+    if (KEPT || g.saved) {
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < RN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            f32x4& at = kept[((i * RN + j) * 4 + q) * NT];
+            if constexpr (KEPT) {
+              const f32x4 v = at;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e];
+            } else {
+              at = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            }
+          }
+    }
+    if constexpr (KEPT) __syncthreads();   // the biases are stored
+  }
   // bf16 backward: the tile of dh passes through registers
   constexpr int DPT = EPI == BWD && SWAP ? BM * BH / 8 / NT : 1;
   s16x8 dh[DPT];
@@ -675,7 +704,7 @@ static int cu_count() {
   return n;
 }
 
-template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
+template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT = false>
 static void launch(TileArgs g, int splits, hipStream_t s) {
   constexpr int BM = 32 * RM * WM, BH = EPI == FWD || EPI == BWD ? 16 * RN * WN : 32 * RN * WN;
   const long tm = tiles(g.M, BM), tn = tiles(g.N, BH);
@@ -685,24 +714,56 @@ static void launch(TileArgs g, int splits, hipStream_t s) {
   g.tn = (int)tn;
   const int all = (int)(tiles(g.K, Elem<T>::STEP) * g.segs);
   g.chunk = (int)tiles(all, splits);
-  hipLaunchKernelGGL((tile_kernel<T, RM, RN, WM, WN, ACOL, BCOL, EPI>), dim3((unsigned)(g.tm * g.tn), (unsigned)tiles(all, g.chunk)),
+  hipLaunchKernelGGL((tile_kernel<T, RM, RN, WM, WN, ACOL, BCOL, EPI, KEPT>), dim3((unsigned)(g.tm * g.tn), (unsigned)tiles(all, g.chunk)),
                      dim3(64 * WM * WN), 0, s, g);
   check_launch();
 }
 
-// 256-row tiles where they fill the CUs, 128-row tiles otherwise.
-static bool large(long M, long N, long bn) { return tiles(M, 256) * tiles(N, bn) >= cu_count(); }
-static int pair_rows(long M, long F) { return large(M, F, 128) ? 256 : 128; }
+// Rows of a product's tiles (M x N results, bn columns to 256 rows): 256 where those fill the CUs, 128 otherwise, and for
+// fp32 64 where 128 x 128 tiles leave CUs idle (a step of one keeps a CU's matrix cores 4096 cycles; dx and dW of
+// 2500 x 120 x 520: 30 us on 128 rows, 19 us on 64; large products need the larger tiles' reuse: 64 x 64 alone would read
+// 9 TB/s).
+static int tile_rows(int bf, long M, long N, long bn) {
+  if (tiles(M, 256) * tiles(N, bn) >= cu_count()) return 256;
+  return bf || tiles(M, 128) * tiles(N, bn / 2) >= cu_count() ? 128 : 64;
+}
+static int pair_rows(int bf, long M, long F) { return tile_rows(bf, M, F, 128); }
 // Partial rows of the bias gradient: two wave rows a tile.
-static long part_rows(long M, long F) { return 2 * tiles(M, pair_rows(M, F)); }
+static long part_rows(int bf, long M, long F) { return 2 * tiles(M, pair_rows(bf, M, F)); }
 
 // Most rows of the few-rows kernel.
 constexpr long kRows = 32;
 
-template <class T, int EPI>
+// Whether the forward pass keeps its products: 8 bytes a result written and read again at 4.7 TB/s against 4 D operations
+// at 1.15 PFLOP/s (bf16) or 0.13 (fp32): from D = 1,000 or 110.  (8192 x 2048 x 8192: backward pair 557 us recomputing,
+// 230 us from the kept products, forward 473 -> 546 us; 25600 x 256 x 1024: 90 us recomputing.)
+static bool saves(int bf, long M, long D) { return D >= (bf ? 1024 : 128) && !(bf && M <= kRows); }
+
+// fp32 elements of the kept products, 0 where nothing is kept.
+long saved_elements(int bf, long M, long D, long F) {
+  if (!saves(bf, M, D)) return 0;
+  const int r = pair_rows(bf, M, F);
+  return tiles(M, r) * r * tiles(F, r == 256 ? 128 : 64) * (r == 256 ? 256 : 128);
+}
+
+template <class T, int EPI, bool KEPT = false>
 static void pair(const TileArgs& g, hipStream_t s) {
-  if (pair_rows(g.M, g.N) == 256) launch<T, 4, 2, 2, 4, false, false, EPI>(g, 1, s);
-  else launch<T, 2, 2, 2, 2, false, false, EPI>(g, 1, s);
+  switch (pair_rows(sizeof(T) == 2, g.M, g.N)) {
+    case 256: launch<T, 4, 2, 2, 4, false, false, EPI, KEPT>(g, 1, s); break;
+    case 128: launch<T, 2, 2, 2, 2, false, false, EPI, KEPT>(g, 1, s); break;
+    default:
+      if constexpr (sizeof(T) == 4) launch<T, 1, 2, 2, 2, false, false, EPI, KEPT>(g, 1, s);
+  }
+}
+// The plain products on the same tiles.
+template <class T, bool ACOL, bool BCOL, int EPI>
+static void product(const TileArgs& g, int rows, int splits, hipStream_t s) {
+  switch (rows) {
+    case 256: launch<T, 4, 2, 2, 4, ACOL, BCOL, EPI>(g, splits, s); break;
+    case 128: launch<T, 2, 2, 2, 2, ACOL, BCOL, EPI>(g, splits, s); break;
+    default:
+      if constexpr (sizeof(T) == 4) launch<T, 1, 1, 2, 2, ACOL, BCOL, EPI>(g, splits, s);
+  }
 }
 
 static TileArgs pair_args(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, long M, long D,
@@ -725,11 +786,13 @@ static TileArgs pair_args(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, 
   return g;
 }
 
-void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h, long M, long D,
-             long F, int act, uintptr_t stream) {
+void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h, uintptr_t saved,
+             long M, long D, long F, int act, uintptr_t stream) {
   TileArgs g = pair_args(x, ldx, w, ldw, bf, bias, bias_bf, M, D, F, act);
   g.out = ptr<void>(h);
   g.ldo = F;
+  g.saved = ptr<float>(saved);
+  GSC_CHECK(!saved || saves(bf, M, D), "gated_linear: these products are not kept");
   if (bf && M <= kRows) {
     by_act<true>(act, [&](auto a) {
       constexpr int ACT = decltype(a)::value;
@@ -756,16 +819,12 @@ void pad(uintptr_t src, long lds_, uintptr_t dst, long ldd, int bf, long rows, l
   check_launch();
 }
 
-// fp32 elements of the bias gradient's partial sums.
-long bias_workspace(long M, long F) { return part_rows(M, F) * 2 * F; }
-
 // dgu rows [dg, zeros to a multiple of 8 | du, zeros] from x, the weights and dh; part (absent: no bias gradient) takes
 // the column sums' partial rows.
-void backward_pair(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t dh, long lddh,
-                   uintptr_t dgu, uintptr_t part, uintptr_t db, int db_bf, long M, long D, long F, int act,
+static void backward_pair(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t dh, long lddh,
+                   uintptr_t dgu, uintptr_t part, uintptr_t db, int db_bf, uintptr_t saved, long M, long D, long F, int act,
                    uintptr_t stream) {
   TileArgs g = pair_args(x, ldx, w, ldw, bf, bias, bias_bf, M, D, F, act);
-  GSC_CHECK(!db || part, "gated_linear: the bias gradient needs a workspace");
   if (bf) check_operand(dh, lddh);
   const hipStream_t s = stream_of(stream);
   g.dh = ptr<const void>(dh);
@@ -774,16 +833,23 @@ void backward_pair(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr
   g.half = up8(F);
   g.ldo = 2 * g.half;
   g.part = db ? ptr<float>(part) : nullptr;
-  if (bf) pair<bf16, BWD>(g, s);
-  else pair<float, BWD>(g, s);
+  g.saved = ptr<float>(saved);
+  GSC_CHECK((saved != 0) == (saved_elements(bf, M, D, F) != 0), "gated_linear: the kept products of the forward pass");
+  if (saved) {
+    if (bf) pair<bf16, BWD, true>(g, s);
+    else pair<float, BWD, true>(g, s);
+  } else {
+    if (bf) pair<bf16, BWD>(g, s);
+    else pair<float, BWD>(g, s);
+  }
   if (db) {
     hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)tiles(2 * F, 16)), dim3(256), 0, s, ptr<const float>(part),
-                       part_rows(M, F), 2 * F, ptr<void>(db), db_bf);
+                       part_rows(bf, M, F), 2 * F, ptr<void>(db), db_bf);
     check_launch();
   }
 }
 
-// Splits of a product's K (t tiles of 128 x 128, `outputs` results): n splits divide the time of a tile's steps (0.7 us
+// Splits of a product's K (t tiles, `outputs` results): n splits divide the time of a tile's steps (0.7 us
 // each, of 64) by n and cost n fp32 results written and read again (4 TB/s): the n where the two are equal, two workgroups
 // per CU and at least 4 steps each.  dX of 256 / 2560 rows of 256 x 1024: 22.5 / 22.8 us unsplit, 10.8 / 17 us split;
 // of 25,600 rows 40 us unsplit, 58 us in two.
@@ -792,14 +858,10 @@ static int k_splits(long t, long K, long outputs) {
   return (int)std::max<long>(1, std::min<long>({(long)(n + 0.5), (2L * cu_count() + t - 1) / t, K / 256, 64}));
 }
 
-static int x_splits(long M, long D, long F) {
-  return large(M, D, 256) ? 1 : k_splits(tiles(M, 128) * tiles(D, 128), 2 * F, M * D);
+static int x_splits(int bf, long M, long D, long F) {
+  const int r = tile_rows(bf, M, D, 256);
+  return r == 256 ? 1 : k_splits(tiles(M, r) * tiles(D, r), 2 * F, M * D);
 }
-long x_workspace(long M, long D, long F) {
-  const int n = x_splits(M, D, F);
-  return n > 1 ? n * M * D : 0;
-}
-
 static void add_splits(uintptr_t slabs, const TileArgs& g, int bf, int splits, long n, uintptr_t out, int out_bf, hipStream_t s) {
   const long all = tiles(g.K, bf ? 64 : 32) * g.segs;
   hipLaunchKernelGGL(splits_kernel, dim3(flat_grid(n)), dim3(256), 0, s, ptr<const float>(slabs), n,
@@ -807,14 +869,13 @@ static void add_splits(uintptr_t slabs, const TileArgs& g, int bf, int splits, l
   check_launch();
 }
 
-void backward_x(uintptr_t dgu, uintptr_t w, long ldw, int bf, uintptr_t dx, int dx_bf, uintptr_t slabs, long M, long D, long F,
+static void backward_x(uintptr_t dgu, uintptr_t w, long ldw, int bf, uintptr_t dx, int dx_bf, uintptr_t slabs, long M, long D, long F,
                 uintptr_t stream) {
   check_sizes(M, D, F, 0);
   const hipStream_t s = stream_of(stream);
   check_operand(dgu, 2 * up8(F));
   check_operand(w, ldw);
-  const int es = bf ? 2 : 4, splits = x_splits(M, D, F);
-  GSC_CHECK(splits == 1 || slabs, "gated_linear: the input gradient needs a workspace");
+  const int es = bf ? 2 : 4, splits = x_splits(bf, M, D, F);
   GSC_CHECK(bf || !dx_bf, "gated_linear: fp32 operands give fp32 gradients");
   TileArgs g{};
   g.a[0] = ptr<const void>(dgu);
@@ -830,37 +891,25 @@ void backward_x(uintptr_t dgu, uintptr_t w, long ldw, int bf, uintptr_t dx, int 
   g.out = ptr<void>(splits > 1 ? slabs : dx);
   g.ldo = D;
   g.slab = M * D;
-  const bool big = large(M, D, 256), sum = splits > 1 || !dx_bf;
-  if (!bf) {
-    if (big) launch<float, 4, 2, 2, 4, false, true, SUM>(g, splits, s);
-    else launch<float, 2, 2, 2, 2, false, true, SUM>(g, splits, s);
-  } else if (sum) {
-    if (big) launch<bf16, 4, 2, 2, 4, false, true, SUM>(g, splits, s);
-    else launch<bf16, 2, 2, 2, 2, false, true, SUM>(g, splits, s);
-  } else {
-    if (big) launch<bf16, 4, 2, 2, 4, false, true, OUT>(g, splits, s);
-    else launch<bf16, 2, 2, 2, 2, false, true, OUT>(g, splits, s);
-  }
+  const int rows = tile_rows(bf, M, D, 256);
+  if (!bf) product<float, false, true, SUM>(g, rows, splits, s);
+  else if (splits > 1 || !dx_bf) product<bf16, false, true, SUM>(g, rows, splits, s);
+  else product<bf16, false, true, OUT>(g, rows, splits, s);
   if (splits > 1) add_splits(slabs, g, bf, splits, M * D, dx, dx_bf, s);
 }
 
-static int w_splits(long M, long D, long F) {
-  return large(2 * F, D, 256) ? 1 : k_splits(2 * tiles(F, 128) * tiles(D, 128), M, 2 * F * D);
+static int w_splits(int bf, long M, long D, long F) {
+  const int r = tile_rows(bf, 2 * F, D, 256);
+  return r == 256 ? 1 : k_splits(2 * tiles(F, r) * tiles(D, r), M, 2 * F * D);
 }
 
-long w_workspace(long M, long D, long F) {
-  const int n = w_splits(M, D, F);
-  return n > 1 ? n * 2 * F * D : 0;
-}
-
-void backward_w(uintptr_t dgu, uintptr_t x, long ldx, int bf, uintptr_t dw, int dw_bf, uintptr_t slabs, long M, long D, long F,
+static void backward_w(uintptr_t dgu, uintptr_t x, long ldx, int bf, uintptr_t dw, int dw_bf, uintptr_t slabs, long M, long D, long F,
                 uintptr_t stream) {
   check_sizes(M, D, F, 0);
   const hipStream_t s = stream_of(stream);
   check_operand(dgu, 2 * up8(F));
   check_operand(x, ldx);
-  const int splits = w_splits(M, D, F);
-  GSC_CHECK(splits == 1 || slabs, "gated_linear: the weight gradient needs a workspace");
+  const int splits = w_splits(bf, M, D, F);
   GSC_CHECK(bf || !dw_bf, "gated_linear: fp32 operands give fp32 gradients");
   TileArgs g{};
   g.a[0] = ptr<const void>(dgu);
@@ -876,18 +925,42 @@ void backward_w(uintptr_t dgu, uintptr_t x, long ldx, int bf, uintptr_t dw, int 
   g.ldo = D;
   g.slab = 2 * F * D;
   g.out = ptr<void>(splits > 1 ? slabs : dw);
-  const bool big = large(2 * F, D, 256), sum = splits > 1 || !dw_bf;
-  if (!bf) {
-    if (big) launch<float, 4, 2, 2, 4, true, true, SUM>(g, splits, s);
-    else launch<float, 2, 2, 2, 2, true, true, SUM>(g, splits, s);
-  } else if (sum) {
-    if (big) launch<bf16, 4, 2, 2, 4, true, true, SUM>(g, splits, s);
-    else launch<bf16, 2, 2, 2, 2, true, true, SUM>(g, splits, s);
-  } else {
-    if (big) launch<bf16, 4, 2, 2, 4, true, true, OUT>(g, splits, s);
-    else launch<bf16, 2, 2, 2, 2, true, true, OUT>(g, splits, s);
-  }
+  const int rows = tile_rows(bf, 2 * F, D, 256);
+  if (!bf) product<float, true, true, SUM>(g, rows, splits, s);
+  else if (splits > 1 || !dw_bf) product<bf16, true, true, SUM>(g, rows, splits, s);
+  else product<bf16, true, true, OUT>(g, rows, splits, s);
   if (splits > 1) add_splits(slabs, g, bf, splits, 2 * F * D, dw, dw_bf, s);
+}
+
+// The backward pass's workspace: dgu, the bias gradient's partial sums, and the partial results of dx and dW, which one
+// stretch serves in turn.  Offsets in bytes.
+struct Space {
+  long part, slabs, size;
+};
+static Space space_of(int bf, long M, long D, long F, bool need_x, bool need_w, bool need_b) {
+  auto up = [](long n) { return (n + 255) / 256 * 256; };
+  const int xs = need_x ? x_splits(bf, M, D, F) : 1, ws = need_w ? w_splits(bf, M, D, F) : 1;
+  Space sp;
+  sp.part = up(M * 2 * up8(F) * (bf ? 2 : 4));
+  sp.slabs = sp.part + (need_b ? up(part_rows(bf, M, F) * 2 * F * 4) : 0);
+  sp.size = sp.slabs + 4 * std::max(xs > 1 ? xs * M * D : 0, ws > 1 ? ws * 2 * F * D : 0);
+  return sp;
+}
+long workspace(int bf, long M, long D, long F, bool need_x, bool need_w, bool need_b) {
+  check_sizes(M, D, F, 0);
+  return space_of(bf, M, D, F, need_x, need_w, need_b).size;
+}
+
+// dx, dw, db (0: not asked for) from x, the weights, dh and the kept products (0: computed again).
+void backward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t dh, long lddh,
+              uintptr_t saved, uintptr_t dx, int dx_bf, uintptr_t dw, int dw_bf, uintptr_t db, int db_bf, uintptr_t work,
+              long M, long D, long F, int act, uintptr_t stream) {
+  GSC_CHECK(work, "gated_linear: the backward pass needs a workspace");
+  const Space sp = space_of(bf, M, D, F, dx != 0, dw != 0, db != 0);
+  const uintptr_t dgu = work, slabs = work + sp.slabs;
+  backward_pair(x, ldx, w, ldw, bf, bias, bias_bf, dh, lddh, dgu, work + sp.part, db, db_bf, saved, M, D, F, act, stream);
+  if (dx) backward_x(dgu, w, ldw, bf, dx, dx_bf, slabs, M, D, F, stream);
+  if (dw) backward_w(dgu, x, ldx, bf, dw, dw_bf, slabs, M, D, F, stream);
 }
 
 }  // namespace gated
@@ -895,12 +968,9 @@ void backward_w(uintptr_t dgu, uintptr_t x, long ldx, int bf, uintptr_t dw, int 
 void register_gated(py::module_& m) {
   m.def("gated_forward", &gated::forward, "h = act(x Wg^T + bg) * (x Wu^T + bu)");
   m.def("gated_pad", &gated::pad, "rows copied to a padded row length, zeros behind them");
-  m.def("gated_bias_workspace", &gated::bias_workspace, "fp32 elements of the bias gradient's partial sums");
-  m.def("gated_input_workspace", &gated::x_workspace, "fp32 elements of the input gradient's partial results");
-  m.def("gated_weight_workspace", &gated::w_workspace, "fp32 elements of the weight gradient's partial results");
-  m.def("gated_backward_pair", &gated::backward_pair, "dgu = [dh u act'(g) | dh act(g)] and the bias gradient");
-  m.def("gated_backward_x", &gated::backward_x, "dx = dgu W");
-  m.def("gated_backward_w", &gated::backward_w, "dW = dgu^T x");
+  m.def("gated_workspace", &gated::workspace, "bytes of the backward pass's workspace");
+  m.def("gated_backward", &gated::backward, "dx, dW and the bias gradient");
+  m.def("gated_saved_elements", &gated::saved_elements, "fp32 elements of the products the forward pass keeps (0: none)");
 }
 
 }  // namespace gsc

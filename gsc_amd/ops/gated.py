@@ -3,8 +3,9 @@
     h = act(x Wg^T + bg) * (x Wu^T + bu)        weight [2F, D]: Wg rows over Wu rows, bias [2F]: bg, bu
 
 ``gated_linear`` runs both projections, the activation and the product in one HIP kernel for CUDA tensors, and
-:func:`gated_linear_reference` otherwise.  Operands are bf16 or fp32 with fp32 accumulation; nothing but ``x`` is kept for
-the backward pass, which recomputes both projections and takes every derivative from fp32 values.
+:func:`gated_linear_reference` otherwise.  Operands are bf16 or fp32 with fp32 accumulation.  The backward pass takes every
+derivative from the fp32 values of both projections: it computes them again from ``x``, or, from ``D`` = 1,024 (bf16) or 128
+(fp32) on, where that costs more than memory, reads what the forward pass kept (8 bytes for each element of ``h``).
 
 * bf16 ``x`` with fp32 masters: the weight operand is the masters' bf16 shadow (``FlatParams``) or a cast; their gradients
   come back in fp32.  Under autocast fp32 ``x`` is cast the same way, like :func:`gsc_amd.ops.linear.linear`.
@@ -45,13 +46,13 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def _forward(x2, w, bias, act, D):
+def _forward(x2, w, bias, act, D, saved=None):
     M = x2.shape[0]
     Fo = w.shape[0] // 2
     h = torch.empty(M, Fo, device=x2.device, dtype=x2.dtype)
     if M > 0:
         launch(load_native().gated_forward, x2, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), is_bf16(x2), ptr(bias),
-               is_bf16(bias), h.data_ptr(), M, D, Fo, act)
+               is_bf16(bias), h.data_ptr(), ptr(saved), M, D, Fo, act)
     return h
 
 
@@ -60,45 +61,39 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, w, act, dtype):
         D = x.shape[-1]
         x2, w = _operand(rows_of(x, D).to(dtype)), _operand(w)
-        h = _forward(x2, w, bias, act, D)
-        ctx.save_for_backward(x2, w, bias)
-        nat, M, Fo = load_native(), x2.shape[0], h.shape[1]
+        nat, M, Fo, bf = load_native(), x2.shape[0], w.shape[0] // 2, is_bf16(x2)
+        n = nat.gated_saved_elements(bf, M, D, Fo) if M else 0
+        saved = torch.empty(n, device=x2.device) if n else None
+        h = _forward(x2, w, bias, act, D, saved)
+        ctx.save_for_backward(x2, w, bias, saved)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        ctx.nat, ctx.act, ctx.dev, ctx.x, ctx.w_dtype = nat, act, x.get_device(), (x.shape, x.dtype), weight.dtype
-        ctx.sizes = (M, D, Fo)
-        ctx.space = (nat.gated_input_workspace(M, D, Fo) if M and need_x else 0,
-                     nat.gated_weight_workspace(M, D, Fo) if M and need_w else 0,
-                     nat.gated_bias_workspace(M, Fo) if M and need_b else 0)
+        ctx.run, ctx.dev = nat.gated_backward, x.get_device()
+        ctx.sizes, ctx.flags = (M, D, Fo, x.shape), (bf, is_bf16(bias), act)
+        ctx.types = (x.dtype if need_x else None, weight.dtype if need_w else None, bias.dtype if need_b else None)
+        ctx.space = nat.gated_workspace(bf, M, D, Fo, need_x, need_w, need_b) if M else 0
         return h.view(*x.shape[:-1], Fo)
 
     @staticmethod
     @differentiable_once
     def backward(ctx, dh):
-        x2, w, bias = ctx.saved_tensors
-        (shape, x_dtype), (M, D, Fo), space = ctx.x, ctx.sizes, ctx.space
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev, bf = x2.device, is_bf16(x2)
-        dx = torch.empty(M, D, device=dev, dtype=x_dtype) if need_x else None
-        dw = torch.empty(2 * Fo, D, device=dev, dtype=ctx.w_dtype) if need_w else None
-        db = torch.empty(2 * Fo, device=dev, dtype=bias.dtype) if need_b else None
+        x2, w, bias, saved = ctx.saved_tensors
+        (M, D, Fo, shape), (bf, b_bf, act), (xt, wt, bt) = ctx.sizes, ctx.flags, ctx.types
+        dev = x2.device
+        dx = torch.empty(M, D, device=dev, dtype=xt) if xt is not None else None
+        dw = torch.empty(2 * Fo, D, device=dev, dtype=wt) if wt is not None else None
+        db = torch.empty(2 * Fo, device=dev, dtype=bt) if bt is not None else None
         if M == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
         else:
-            nat, s = ctx.nat, raw_stream(ctx.dev)
             dh2 = rows_of(dh, Fo).to(x2.dtype)
             dh2 = _operand(dh2) if bf else dh2
-            dgu = torch.empty(M, 2 * (-(-Fo // 8) * 8), device=dev, dtype=x2.dtype)
-            xp, wp, gp, xl, wl = x2.data_ptr(), w.data_ptr(), dgu.data_ptr(), x2.stride(0), w.stride(0)
-            work = [torch.empty(n, device=dev) if n else None for n in space]
-            nat.gated_backward_pair(xp, xl, wp, wl, bf, ptr(bias), is_bf16(bias), dh2.data_ptr(), dh2.stride(0), gp,
-                                    ptr(work[2]), ptr(db), is_bf16(db), M, D, Fo, ctx.act, s)
-            if need_x:
-                nat.gated_backward_x(gp, wp, wl, bf, dx.data_ptr(), is_bf16(dx), ptr(work[0]), M, D, Fo, s)
-            if need_w:
-                nat.gated_backward_w(gp, xp, xl, bf, dw.data_ptr(), is_bf16(dw), ptr(work[1]), M, D, Fo, s)
-        return dx.view(shape) if need_x else None, dw, db, None, None, None
+            work = torch.empty(ctx.space, device=dev, dtype=torch.uint8)
+            ctx.run(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), bf, ptr(bias), b_bf, dh2.data_ptr(), dh2.stride(0),
+                    ptr(saved), ptr(dx), xt is torch.bfloat16, ptr(dw), wt is torch.bfloat16, ptr(db), bt is torch.bfloat16,
+                    work.data_ptr(), M, D, Fo, act, raw_stream(ctx.dev))
+        return dx.view(shape) if dx is not None else None, dw, db, None, None, None
 
 
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "silu",
