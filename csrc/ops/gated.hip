@@ -496,8 +496,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
         sg += __shfl_xor(sg, 32);
         su += __shfl_xor(su, 32);
         if (lane < 32 && in) {
-          g.part[(long)part_row * 2 * g.N + n] = sg;
-          g.part[(long)part_row * 2 * g.N + g.N + n] = su;
+          g.part[(long)part_row * 2 * g.half + n] = sg;
+          g.part[(long)part_row * 2 * g.half + g.half + n] = su;
         }
       }
     }
@@ -557,12 +557,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
         if (EPI == BWD && g.part) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float a = half_wave_sum(sg[e]), b = half_wave_sum(su[e]);
-            const long n = n0 + col + e;
-            if ((lane & 31) == 31 && n < g.N) {
-              g.part[(long)part_row * 2 * g.N + n] = a;
-              g.part[(long)part_row * 2 * g.N + g.N + n] = b;
-            }
+            sg[e] = half_wave_sum(sg[e]);
+            su[e] = half_wave_sum(su[e]);
+          }
+          if ((lane & 31) == 31 && n0 + col < g.half) {
+            float* row = g.part + (long)part_row * 2 * g.half + n0 + col;
+            *reinterpret_cast<f32x4*>(row) = f32x4{sg[0], sg[1], sg[2], sg[3]};
+            *reinterpret_cast<f32x4*>(row + g.half) = f32x4{su[0], su[1], su[2], su[3]};
           }
         }
       }
@@ -663,17 +664,20 @@ __global__ __launch_bounds__(256) void splits_kernel(const float* slabs, long sl
   }
 }
 
-// out[c] = sum over the partial rows: 16 columns x 16 row phases a workgroup, phases added in order.
-__global__ __launch_bounds__(256) void colsum_kernel(const float* part, long rows, long C, void* out, int out_bf) {
+// out[c] = sum over the partial rows [gate F, padding | up F, padding]: 16 columns x 16 row phases a workgroup, phases added
+// in order.
+__global__ __launch_bounds__(256) void colsum_kernel(const float* part, long rows, long F, long half, void* out, int out_bf) {
   __shared__ float red[16][17];
   const int cl = threadIdx.x & 15, ph = threadIdx.x >> 4;
-  const long c = (long)blockIdx.x * 16 + cl;
+  const long c = (long)blockIdx.x * 16 + cl, at = c < F ? c : c - F + half;
   float s = 0.f;
-  if (c < C)
-    for (long z = ph; z < rows; z += 16) s += part[z * C + c];
+  if (c < 2 * F) {
+#pragma unroll 4
+    for (long z = ph; z < rows; z += 16) s += part[z * 2 * half + at];
+  }
   red[ph][cl] = s;
   __syncthreads();
-  if (ph || c >= C) return;
+  if (ph || c >= 2 * F) return;
 #pragma unroll
   for (int q = 1; q < 16; ++q) s += red[q][cl];
   if (out_bf) reinterpret_cast<bf16*>(out)[c] = __float2bfloat16(s);
@@ -844,7 +848,7 @@ static void backward_pair(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, 
   }
   if (db) {
     hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)tiles(2 * F, 16)), dim3(256), 0, s, ptr<const float>(part),
-                       part_rows(bf, M, F), 2 * F, ptr<void>(db), db_bf);
+                       part_rows(bf, M, F), F, g.half, ptr<void>(db), db_bf);
     check_launch();
   }
 }
@@ -942,7 +946,7 @@ static Space space_of(int bf, long M, long D, long F, bool need_x, bool need_w, 
   const int xs = need_x ? x_splits(bf, M, D, F) : 1, ws = need_w ? w_splits(bf, M, D, F) : 1;
   Space sp;
   sp.part = up(M * 2 * up8(F) * (bf ? 2 : 4));
-  sp.slabs = sp.part + (need_b ? up(part_rows(bf, M, F) * 2 * F * 4) : 0);
+  sp.slabs = sp.part + (need_b ? up(part_rows(bf, M, F) * 2 * up8(F) * 4) : 0);
   sp.size = sp.slabs + 4 * std::max(xs > 1 ? xs * M * D : 0, ws > 1 ? ws * 2 * F * D : 0);
   return sp;
 }
