@@ -93,3 +93,23 @@ def test_refused_values(call):
 def test_refused_types(call):
     with pytest.raises(TypeError):
         call(torch.zeros(3, 4))
+
+
+def test_native_refusals():
+    """What the kernels cannot address is refused on the host, before any launch."""
+    nat = pytest.importorskip("gsc_amd.native").load()
+    assert nat.gated_workspace(True, 100, 64, 256, True, True, True) >= 100 * 512 * 2
+    for sizes in ((0, 8, 8), (8, 0, 8), (8, 8, 0), (8, 1_000_001, 8), (8, 8, 1_000_001), (1 << 31, 8, 8)):
+        with pytest.raises(RuntimeError, match="gated_linear"):
+            nat.gated_workspace(True, *sizes, True, True, True)
+    call = lambda x, ldx: nat.gated_forward(x, ldx, 256, 8, True, 0, False, 256, 0, 4, 8, 4, 0, 0)
+    for x, ldx in ((264, 8), (256, 12), (256, 2_000_008)):   # unaligned rows, rows too long for a descriptor
+        with pytest.raises(RuntimeError, match="16-byte aligned rows"):
+            call(x, ldx)
+    with pytest.raises(RuntimeError, match="activation"):
+        nat.gated_forward(256, 8, 256, 8, True, 0, False, 256, 0, 4, 8, 4, 3, 0)
+    with pytest.raises(RuntimeError, match="layer_norm"):
+        nat.layer_norm_forward(256, 8, True, 0, False, 0, False, 256, 0, 0, 0, 8, 1e-5, 0)
+    for p in (1.0, -0.5, float("nan")):
+        with pytest.raises(RuntimeError, match="dropout"):
+            nat.dropout(256, 0, 256, True, 8, 1, 1, 0, 0, p, 0)

@@ -259,7 +259,8 @@ def _blocks_at(groups, seed, offset):
 
 GATED_SHAPES = [(1, 1, 1), (1, 256, 1024), (2, 8, 5), (3, 100, 33), (8, 512, 96), (16, 64, 64), (33, 72, 40), (64, 22, 256),
                 (65, 257, 129), (100, 64, 256), (130, 96, 200), (257, 264, 136), (300, 31, 77), (600, 320, 512),
-                (1100, 128, 640), (4200, 72, 2101), (4200, 4104, 72), (100, 4104, 2104)]
+                (1100, 128, 640), (4200, 72, 2101), (4200, 4104, 72), (100, 4104, 2104), (40, 1032, 72),
+                (200, 1100, 130), (2200, 1024, 1100), (90, 128, 64)]
 
 
 def _gated_check(x, w, b, dh, act, op, w_used=None):
@@ -507,6 +508,66 @@ def test_capture_refused_while_an_eager_graph_of_the_leaves_lives():
         gr.replay()
         assert torch.equal(got, want)
         del y, got, gr
+
+
+def _each(g):
+    """A call of each operator on fresh leaves, and the leaves."""
+    x, w, gw = (_randn(g, 20, 32).requires_grad_(), _randn(g, 32, shift=1.0).requires_grad_(),
+                _randn(g, 16, 32).requires_grad_())
+    return [(lambda: ops.layer_norm(x, w), (x, w)), (lambda: ops.dropout(x, 0.5, 3, 1), (x,)),
+            (lambda: ops.gated_linear(x, gw), (x, gw))]
+
+
+def test_graph_kept_for_a_second_backward_pass():
+    for call, leaves in _each(_gen(41)):
+        y = call()
+        dy = torch.ones_like(y)
+        first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, leaves, dy)))
+
+
+def test_second_derivatives_are_refused():
+    """A gradient taken with create_graph is right, and differentiating it again raises instead of giving zeros."""
+    for call, leaves in _each(_gen(42)):
+        y = call()
+        plain = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
+        dy = torch.ones_like(y).requires_grad_()
+        grads = torch.autograd.grad(y, leaves, dy, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            grads[0].sum().backward()
+
+
+def test_inputs_changed_before_the_backward_pass_are_noticed():
+    g = _gen(43)
+    x, w = _randn(g, 20, 32), _randn(g, 32, shift=1.0).requires_grad_()
+    gw = _randn(g, 16, 32).requires_grad_()
+    for call, leaf in ((lambda: ops.layer_norm(x, w), w), (lambda: ops.gated_linear(x, gw), gw)):
+        y = call()
+        x.add_(1.0)
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(y, leaf, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gated_linear_kept_products_equal_recomputed_ones(dtype):
+    """On both sides of the widths from which the forward pass keeps its products: the same bounds hold, and a wider
+    operand padded with zeros gives the same gradients as the narrow one."""
+    g = _gen(44)
+    D = 1016 if dtype == BF16 else 120
+    x, w, b, dh = _gated_inputs(g, 150, D, 72, dtype)
+    pad = lambda t: torch.cat([t, torch.zeros(t.shape[0], 8, device="cuda", dtype=t.dtype)], 1)
+    out = []
+    for xx, ww in ((x, w), (pad(x), pad(w))):
+        leaves = [t.detach().requires_grad_() for t in (xx, ww, b)]
+        h = ops.gated_linear(*leaves, activation="gelu")
+        out.append([h.detach(), *torch.autograd.grad(h, leaves, dh)])
+    (h, dx, dw, db), (h2, dx2, dw2, db2) = out
+    want = gated_bounds(x, w, b, dh, "gelu", dtype)
+    for name, a, c in (("h", h, h2), ("dx", dx, dx2[:, :D]), ("dw", dw, dw2[:, :D]), ("db", db, db2)):
+        close(name, a, *want[name], dtype)
+        close(name, c, *want[name], dtype)
+    assert not dw2[:, D:].any()
 
 
 def test_refused_on_the_gpu():
