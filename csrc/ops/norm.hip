@@ -473,11 +473,12 @@ void forward(uintptr_t x, long ldx, int bf, uintptr_t w, int w_bf, uintptr_t b, 
 }
 
 // fp32 elements of the backward's partial column sums, whatever its operands' alignment.
-long workspace(long M, long C, int bf) {
+static long workspace(long M, long C, int bf) {
+  check_sizes(M, C);
   return 2 * C * std::max(parts_of(M, C, bf ? 8 : 4), parts_of(M, C, 1));
 }
 
-void backward(uintptr_t x, long ldx, uintptr_t dy, long lddy, int bf, uintptr_t w, int w_bf, uintptr_t mean, uintptr_t rstd,
+static void backward(uintptr_t x, long ldx, uintptr_t dy, long lddy, int bf, uintptr_t w, int w_bf, uintptr_t mean, uintptr_t rstd,
               uintptr_t dx, uintptr_t dw, int dw_bf, uintptr_t db, int db_bf, uintptr_t part, long M, long C,
               uintptr_t stream) {
   check_sizes(M, C);
@@ -498,12 +499,29 @@ void backward(uintptr_t x, long ldx, uintptr_t dy, long lddy, int bf, uintptr_t 
   }
 }
 
+// A backward pass prepared by its forward pass: what is known then, and the call with the rest (0: not asked for).
+struct Backward {
+  int bf, w_bf;
+  uintptr_t stats;   // mean [M], 1/std [M]
+  long M, C;
+  int dw_bf, db_bf;
+  long space;        // fp32 elements of its workspace
+  Backward(int bf, int w_bf, uintptr_t stats, long M, long C, int dw_bf, int db_bf)
+      : bf(bf), w_bf(w_bf), stats(stats), M(M), C(C), dw_bf(dw_bf), db_bf(db_bf), space(workspace(M, C, bf)) {}
+  void run(uintptr_t x, long ldx, uintptr_t dy, long lddy, uintptr_t w, uintptr_t dx, uintptr_t dw, uintptr_t db,
+           uintptr_t part, uintptr_t stream) const {
+    backward(x, ldx, dy, lddy, bf, w, w_bf, stats, stats + 4 * M, dx, dw, dw_bf, db, db_bf, part, M, C, stream);
+  }
+};
+
 }  // namespace norm
 
 void register_norm(py::module_& m) {
   m.def("layer_norm_forward", &norm::forward, "layer norm of rows: y, and mean / 1/std per row when asked for");
-  m.def("layer_norm_workspace", &norm::workspace, "fp32 elements the backward's parameter gradients need");
-  m.def("layer_norm_backward", &norm::backward, "layer norm gradients (dx, and dw / db through the workspace)");
+  py::class_<norm::Backward>(m, "LayerNormBackward", "layer norm gradients (dx, and dw / db through the workspace)")
+      .def(py::init<int, int, uintptr_t, long, long, int, int>())
+      .def_readonly("space", &norm::Backward::space)
+      .def("__call__", &norm::Backward::run);
 }
 
 }  // namespace gsc

@@ -46,36 +46,37 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         x2 = rows_of(x, x.shape[-1])
         y, st = _forward(x2, weight, bias, eps, True)
-        ctx.save_for_backward(x2, weight, st)
-        M, C = x2.shape
-        nat, need, bf = load_native(), ctx.needs_input_grad, is_bf16(x2)
-        ctx.sizes, ctx.dev, ctx.run = (M, C, x.shape), x.get_device(), nat.layer_norm_backward
-        ctx.types = (weight.dtype if need[1] else None, bias.dtype if need[2] else None)
-        ctx.flags = (bf, is_bf16(weight))
-        ctx.part = nat.layer_norm_workspace(M, C, bf) if M and (need[1] or need[2]) else 0
+        ctx.save_for_backward(x2, weight)
+        (M, C), need = x2.shape, ctx.needs_input_grad
+        wt, bt = weight.dtype if need[1] else None, bias.dtype if need[2] else None
+        ctx.stats, ctx.shape, ctx.types, ctx.dev, ctx.plan = st, x.shape, (wt, bt), x.get_device(), None
+        if M:
+            ctx.plan = load_native().LayerNormBackward(is_bf16(x2), is_bf16(weight), st.data_ptr(), M, C, wt is torch.bfloat16,
+                                                       bt is torch.bfloat16)
         return y.view(x.shape)
 
     @staticmethod
     @differentiable_once
     def backward(ctx, dy):
-        x2, weight, st = ctx.saved_tensors
-        (M, C, shape), (bf, w_bf), (wt, bt) = ctx.sizes, ctx.flags, ctx.types
-        dev = x2.device
-        dx = torch.empty(M, C, device=dev, dtype=x2.dtype) if ctx.needs_input_grad[0] else None
+        x2, weight = ctx.saved_tensors   # read here: a saved-tensor hook may have moved them
+        plan, (wt, bt), shape, dev = ctx.plan, ctx.types, ctx.shape, x2.device
+        C = shape[-1]
         dw = torch.empty(C, device=dev, dtype=wt) if wt is not None else None
         db = torch.empty(C, device=dev, dtype=bt) if bt is not None else None
-        if M == 0:
+        dx = torch.empty(shape, device=dev, dtype=x2.dtype) if ctx.needs_input_grad[0] else None
+        if plan is None:   # no rows
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
-        else:
-            dy2 = rows_of(dy, C)
-            part = torch.empty(ctx.part, device=dev) if ctx.part else None
-            s0 = st.data_ptr()
-            ctx.run(x2.data_ptr(), x2.stride(0), dy2.data_ptr(), dy2.stride(0), bf, ptr(weight), w_bf, s0, s0 + 4 * M,
-                    ptr(dx), ptr(dw), wt is torch.bfloat16, ptr(db), bt is torch.bfloat16, ptr(part), M, C,
-                    raw_stream(ctx.dev))
-        return dx.view(shape) if dx is not None else None, dw, db, None
+            return dx, dw, db, None
+        part = torch.empty(plan.space, device=dev) if dw is not None or db is not None else None
+        ld = C
+        if not dy.is_contiguous():
+            dy = rows_of(dy, C)
+            ld = dy.stride(0)
+        plan(x2.data_ptr(), x2.stride(0), dy.data_ptr(), ld, ptr(weight), ptr(dx), ptr(dw), ptr(db), ptr(part),
+             raw_stream(ctx.dev))
+        return dx, dw, db, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,

@@ -550,6 +550,36 @@ def test_inputs_changed_before_the_backward_pass_are_noticed():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [31, 1024])
+def test_saved_tensors_moved_to_the_host_or_recomputed(D, dtype):
+    """The gradients are those of a plain call, bit for bit, where a hook moves what a forward pass saved or the forward
+    pass runs again before the backward one."""
+    from torch.utils.checkpoint import checkpoint
+    g = _gen(45, D)
+    x, dy = _randn(g, 60, 2 * D, dtype=dtype)[:, :D], _randn(g, 60, 24, dtype=dtype)
+    w, b = _randn(g, D, shift=1.0), _randn(g, D)
+    gw, gb = _randn(g, 48, D, dtype=dtype, scale=D ** -0.5), _randn(g, 48, dtype=dtype)
+
+    def block(x, w, b, gw, gb):
+        return ops.dropout(ops.gated_linear(ops.layer_norm(x, w, b), gw, gb), 0.3, 5)
+
+    def call(run):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, gw, gb)]
+        y = run(leaves)
+        spoil = torch.full((1 << 16,), float("nan"), device="cuda")   # reuses what the call freed
+        del spoil
+        return torch.autograd.grad(y, leaves, dy)
+
+    def on_host(leaves):
+        with torch.autograd.graph.save_on_cpu():
+            return block(*leaves)
+
+    plain = call(lambda leaves: block(*leaves))
+    for run in (on_host, lambda leaves: checkpoint(block, *leaves, use_reentrant=False, preserve_rng_state=False)):
+        assert all(torch.equal(a, c) for a, c in zip(plain, call(run)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_gated_linear_kept_products_equal_recomputed_ones(dtype):
     """On both sides of the widths from which the forward pass keeps its products: the same bounds hold, and a wider
     operand padded with zeros gives the same gradients as the narrow one."""
