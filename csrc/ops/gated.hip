@@ -712,7 +712,7 @@ template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI
 static void launch(TileArgs g, int splits, hipStream_t s) {
   constexpr int BM = 32 * RM * WM, BH = EPI == FWD || EPI == BWD ? 16 * RN * WN : 32 * RN * WN;
   const long tm = tiles(g.M, BM), tn = tiles(g.N, BH);
-  GSC_CHECK(2 * tm * tn <= 0x7fffffffL, "gated_linear: too many tiles");
+  GSC_CHECK((g.tmh ? 2 : 1) * tm * tn * (64 * WM * WN) <= 0xffffffffL, "gated_linear: too many tiles");   // threads of a grid
   if (g.tmh) g.tmh = (int)tm;
   g.tm = (int)(g.tmh ? 2 * tm : tm);
   g.tn = (int)tn;

@@ -128,13 +128,20 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
   return v;
 }
 
+// Grids of one workgroup per row (or few) have two dimensions: one holds at most 2^32 - 1 threads.
+__device__ __forceinline__ long block_of() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
+static dim3 grid_of(long blocks) {
+  const long x = std::min<long>(blocks, 1L << 20);
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+
 template <class T, int VEC, int G, int N>
 __global__ __launch_bounds__(G > 256 ? G : 256) void fwd_kernel(const T* x, long ldx, Param w, Param b, T* y, float* mean,
                                                                 float* rstd, long M, int C, float eps) {
   constexpr int NT = G > 256 ? G : 256, E = VEC * N;
   __shared__ float red[16];
   const int lane = threadIdx.x % G;
-  const long row0 = (long)blockIdx.x * (NT / G) + threadIdx.x / G, row = row0 < M ? row0 : M - 1;
+  const long row0 = block_of() * (NT / G) + threadIdx.x / G, row = row0 < M ? row0 : M - 1;
   const T* xr = x + row * ldx;
   float v[E];
   float s = 0.f;
@@ -284,9 +291,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void bwd_kernel(const T* x, long
 
 template <class T>
 __global__ __launch_bounds__(1024) void fwd_long_kernel(const T* x, long ldx, Param w, Param b, T* y, float* mean,
-                                                        float* rstd, int C, float eps) {
+                                                        float* rstd, long M, int C, float eps) {
   __shared__ float red[16];
-  const long row = blockIdx.x;
+  const long row = block_of();
+  if (row >= M) return;
   const T* xr = x + row * ldx;
   float s = 0.f;
   for (int c = threadIdx.x; c < C; c += 1024) s += to_f(xr[c]);
@@ -307,9 +315,11 @@ __global__ __launch_bounds__(1024) void fwd_long_kernel(const T* x, long ldx, Pa
 
 template <class T>
 __global__ __launch_bounds__(1024) void bwd_long_kernel(const T* x, long ldx, const T* dy, long lddy, Param w,
-                                                        const float* mean, const float* rstd, T* dx, int C) {
+                                                        const float* mean, const float* rstd, T* dx, long M,
+                                                        int C) {
   __shared__ float red[16];
-  const long row = blockIdx.x;
+  const long row = block_of();
+  if (row >= M) return;
   const T *xr = x + row * ldx, *gr = dy + row * lddy;
   const float mu = mean[row], r = rstd[row];
   float s = 0.f, q = 0.f;
@@ -391,7 +401,7 @@ static int vec_of(uintptr_t x, long ldx, uintptr_t y, long ldy, uintptr_t w, uin
 // Partial rows of the backward: workgroups, each over rows / workgroups rows (at most 1,024, and 8 MB of partial sums or 512).
 static int parts_of(long M, long C, int vec) {
   const Shape sh = shape_of(C, vec);
-  if (!sh.g) return (int)std::max<long>(1, std::min<long>(256, M / 16));
+  if (!sh.g) return (int)std::max<long>(1, std::min<long>({256, M / 16, (1L << 27) / C}));   // at most 1 GB
   const long wg = sh.g > 256 ? 1 : 256 / sh.g;
   return (int)std::max<long>(1, std::min<long>({(M + wg - 1) / wg, 1024, std::max<long>(512, (1L << 21) / (2 * C))}));
 }
@@ -421,12 +431,12 @@ static void run_fwd(uintptr_t x, long ldx, Param w, Param b, uintptr_t y, uintpt
                     float eps, hipStream_t s) {
   const Shape sh = shape_of(C, VEC);
   if (!sh.g) {
-    hipLaunchKernelGGL((fwd_long_kernel<T>), dim3((unsigned)M), dim3(1024), 0, s, ptr<const T>(x), ldx, w, b, ptr<T>(y),
-                       ptr<float>(mean), ptr<float>(rstd), C, eps);
+    hipLaunchKernelGGL((fwd_long_kernel<T>), grid_of(M), dim3(1024), 0, s, ptr<const T>(x), ldx, w, b, ptr<T>(y),
+                       ptr<float>(mean), ptr<float>(rstd), M, C, eps);
   } else {
     by_shape<VEC>(sh, [&](auto g, auto n) {
       constexpr int G = decltype(g)::value, N = decltype(n)::value, NT = G > 256 ? G : 256;
-      hipLaunchKernelGGL((fwd_kernel<T, VEC, G, N>), dim3((unsigned)((M + NT / G - 1) / (NT / G))), dim3(NT), 0, s,
+      hipLaunchKernelGGL((fwd_kernel<T, VEC, G, N>), grid_of((M + NT / G - 1) / (NT / G)), dim3(NT), 0, s,
                          ptr<const T>(x), ldx, w, b, ptr<T>(y), ptr<float>(mean), ptr<float>(rstd), M, C, eps);
     });
   }
@@ -440,8 +450,8 @@ static void run_bwd(uintptr_t x, long ldx, uintptr_t dy, long lddy, Param w, uin
   const int parts = parts_of(M, C, VEC);
   if (!sh.g) {
     if (dx)
-      hipLaunchKernelGGL((bwd_long_kernel<T>), dim3((unsigned)M), dim3(1024), 0, s, ptr<const T>(x), ldx, ptr<const T>(dy),
-                         lddy, w, ptr<const float>(mean), ptr<const float>(rstd), ptr<T>(dx), C);
+      hipLaunchKernelGGL((bwd_long_kernel<T>), grid_of(M), dim3(1024), 0, s, ptr<const T>(x), ldx, ptr<const T>(dy),
+                         lddy, w, ptr<const float>(mean), ptr<const float>(rstd), ptr<T>(dx), M, C);
     if (part)
       hipLaunchKernelGGL((bwd_long_sums_kernel<T>), dim3((C + 255) / 256, parts), dim3(256), 0, s, ptr<const T>(x), ldx,
                          ptr<const T>(dy), lddy, ptr<const float>(mean), ptr<const float>(rstd), ptr<float>(part), M, C);
@@ -457,7 +467,8 @@ static void run_bwd(uintptr_t x, long ldx, uintptr_t dy, long lddy, Param w, uin
 }
 
 static void check_sizes(long M, long C) {
-  GSC_CHECK(M >= 1 && M <= 0x7fffffffL && C >= 1 && C <= 0x7fff0000L, "layer_norm: rows and columns must be in 1 .. 2^31 - 2^16");
+  GSC_CHECK(M >= 1 && M <= 0x7fffffffL && C >= 1 && C <= 1L << 24,
+            "layer_norm: rows must be in 1 .. 2^31 - 1, columns in 1 .. 2^24");
 }
 
 void forward(uintptr_t x, long ldx, int bf, uintptr_t w, int w_bf, uintptr_t b, int b_bf, uintptr_t y, uintptr_t mean,

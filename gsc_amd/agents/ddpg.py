@@ -62,10 +62,10 @@ class DDPGLearner:
         torch.manual_seed(seed)
         self.actor = Actor(cfg, obs_dim, action_dim).to(self.device)
         self.critic = QNetwork(cfg, obs_dim, action_dim).to(self.device)
-        # dropout (a config option) is active only where a network's own loss is taken (_training); each network has its own
-        # masks, a function of the seed and the number of updates
+        # dropout (a config option) is active only where a network's own loss is taken (_training); each network of
+        # each rank has its own masks, a function of the seed and the number of updates
         for k, m in enumerate((self.actor, self.critic)):
-            m.mlp.seed_dropout(seed * 0x5851F42D4C957F2D + k + 1)
+            m.mlp.seed_dropout(seed * 0x5851F42D4C957F2D + 0x2545F4914F6CDD1D * self.dist.rank + k + 1)
             m.eval()
         self.target_actor = copy.deepcopy(self.actor)
         self.target_critic = copy.deepcopy(self.critic)

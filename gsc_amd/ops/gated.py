@@ -19,7 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
+from .launch import check_device, check_types, dense, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
 from .linear import shadow
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
@@ -35,11 +35,11 @@ def gated_linear_reference(x: torch.Tensor, weight: torch.Tensor, bias: Optional
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
-    """The matrix [rows, cols] as the kernels read it: rows start on 16 bytes and end on a multiple of 8 elements (a copy
-    with zeros behind each row where they do not)."""
+    """The matrix [rows, cols] as the kernels read it: rows start on 16 bytes, at most 2,000,000 elements apart, and end on a
+    multiple of 8 elements (a copy with zeros behind each row where they do not)."""
     rows, cols = t.shape
     if rows == 0 or (cols % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-                     and t.stride(0) >= cols):
+                     and cols <= t.stride(0) <= 2_000_000):
         return t
     out = torch.empty(rows, -(-cols // 8) * 8, device=t.device, dtype=t.dtype)
     launch(load_native().gated_pad, t, t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0), is_bf16(t), rows, cols)
@@ -59,7 +59,7 @@ def _forward(x2, w, bias, act, D, saved=None):
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, w, act, dtype):
-        D = x.shape[-1]
+        D, bias = x.shape[-1], dense(bias)
         x2, w = _operand(rows_of(x, D).to(dtype)), _operand(w)
         nat, M, Fo, bf = load_native(), x2.shape[0], w.shape[0] // 2, is_bf16(x2)
         n = nat.gated_saved_elements(bf, M, D, Fo) if M else 0
@@ -127,9 +127,8 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         w = w16 if w16 is not None else shadow(weight)
         w = w if w is not None else weight.detach().to(dtype)
     w = rows_of(w.detach(), D)
-    bias = bias.contiguous() if bias is not None else None
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         h = _GatedLinear.apply(x, weight, bias, w, ACTIVATIONS[activation], dtype)
         return note_leaves("gated_linear", h, x, weight, bias)
-    h = _forward(_operand(rows_of(x, D).to(dtype)), _operand(w), bias, ACTIVATIONS[activation], D)
+    h = _forward(_operand(rows_of(x, D).to(dtype)), _operand(w), dense(bias), ACTIVATIONS[activation], D)
     return h.view(*x.shape[:-1], h.shape[1])

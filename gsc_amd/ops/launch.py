@@ -34,6 +34,11 @@ def rows_of(t: torch.Tensor, C: int) -> torch.Tensor:
     return t if C == 1 or t.stride(1) == 1 else t.contiguous()
 
 
+def dense(t):
+    """``t`` with contiguous elements, None as it is."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def check_device(name: str, x: torch.Tensor, **others) -> None:
     for k, t in others.items():
         if t is not None and t.device != x.device:

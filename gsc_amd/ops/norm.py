@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
+from .launch import check_device, check_types, dense, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
 
 
 def layer_norm_reference(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -45,14 +45,15 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         x2 = rows_of(x, x.shape[-1])
+        weight, bias = dense(weight), dense(bias)
         y, st = _forward(x2, weight, bias, eps, True)
         ctx.save_for_backward(x2, weight)
         (M, C), need = x2.shape, ctx.needs_input_grad
         wt, bt = weight.dtype if need[1] else None, bias.dtype if need[2] else None
         ctx.stats, ctx.shape, ctx.types, ctx.dev, ctx.plan = st, x.shape, (wt, bt), x.get_device(), None
         if M:
-            ctx.plan = load_native().LayerNormBackward(is_bf16(x2), is_bf16(weight), st.data_ptr(), M, C, wt is torch.bfloat16,
-                                                       bt is torch.bfloat16)
+            ctx.plan = load_native().LayerNormBackward(is_bf16(x2), is_bf16(weight), st.data_ptr(), M, C,
+                                                       wt is torch.bfloat16, bt is torch.bfloat16)
         return y.view(x.shape)
 
     @staticmethod
@@ -94,9 +95,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         return layer_norm_reference(x, weight, bias, eps)
     check_types("layer_norm", x=x, weight=weight, bias=bias)
     check_device("layer_norm", x, weight=weight, bias=bias)
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return note_leaves("layer_norm", _LayerNorm.apply(x, weight, bias, float(eps)), x, weight, bias)
-    return _forward(rows_of(x, C), weight, bias, float(eps), False)[0].view(x.shape)
+    return _forward(rows_of(x, C), dense(weight), dense(bias), float(eps), False)[0].view(x.shape)

@@ -6,6 +6,7 @@ import yaml
 from gsc_amd.agents import Batch, DDPGLearner
 from gsc_amd.coordsim.reader import load_topology
 from gsc_amd.models import Actor, GraphSet, MaskedInputMLP, QNetwork, count_params
+from gsc_amd.parallel.dist import DistInfo
 from gsc_amd.utils.checkpoint import load_actor, save_actor
 from tests.conftest import cfg_path
 
@@ -138,6 +139,14 @@ def test_learner_updates_every_part_and_resumes(tmp_path):
     b = _batch(4)
     with torch.no_grad():
         torch.testing.assert_close(actor(b.obs, b.topo, gs, L.masks), L.act(b.obs, b.topo), rtol=0, atol=0)
+
+
+def test_every_rank_draws_its_own_masks():
+    cfg = _cfg(actor_dropout=0.1, critic_dropout=0.2)
+    gs = GraphSet([load_topology(ABILENE)], 24, "cpu")
+    a, b = (DDPGLearner(cfg, 3, 1728, gs, 1, 3, "cpu", DistInfo(rank=r), seed=3) for r in (0, 1))
+    assert torch.equal(a.critic_flat.flat, b.critic_flat.flat)
+    assert len({n.mlp.drop_seed for L in (a, b) for n in (L.actor, L.critic)}) == 4
 
 
 def test_renewed_parameters_keep_storage_and_places():

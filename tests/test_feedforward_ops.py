@@ -113,3 +113,13 @@ def test_native_refusals():
     for p in (1.0, -0.5, float("nan")):
         with pytest.raises(RuntimeError, match="dropout"):
             nat.dropout(256, 0, 256, True, 8, 1, 1, 0, 0, p, 0)
+
+
+def test_native_refusals_of_layer_norm_sizes():
+    nat = pytest.importorskip("gsc_amd.native").load()
+    for M, C in ((0, 8), (8, 0), (1 << 31, 8), (8, (1 << 24) + 1)):
+        with pytest.raises(RuntimeError, match="layer_norm"):
+            nat.layer_norm_forward(256, 8, True, 0, False, 0, False, 256, 0, 0, M, C, 1e-5, 0)
+        with pytest.raises(RuntimeError, match="layer_norm"):
+            nat.LayerNormBackward(True, False, 0, M, C, False, False)
+    assert nat.LayerNormBackward(True, False, 0, 1 << 20, 1 << 24, False, False).space <= 1 << 28   # 1 GB

@@ -600,6 +600,53 @@ def test_gated_linear_kept_products_equal_recomputed_ones(dtype):
     assert not dw2[:, D:].any()
 
 
+def test_layer_norm_more_rows_than_one_grid_dimension_holds():
+    M, C = (1 << 29) + 37, 2   # 8 lanes a row: over 2^32 threads
+    x = torch.zeros(M, C, device="cuda", dtype=BF16)
+    x[-100:] = _randn(_gen(46), 100, C, dtype=BF16)
+    x.requires_grad_()
+    y = ops.layer_norm(x, eps=0.5)
+    (dx,) = torch.autograd.grad(y, x, x.detach())
+    t = x.detach()[-100:].clone().requires_grad_()
+    z = ops.layer_norm(t, eps=0.5)
+    (dt,) = torch.autograd.grad(z, t, t.detach())
+    assert t.any() and torch.equal(y[-100:], z) and torch.equal(dx[-100:], dt)
+    assert not y[:-100].any() and not dx[:-100].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gated_linear_rows_far_apart(dtype):
+    """Rows further apart than a tile can address are copied."""
+    g = _gen(47)
+    for M in (3, 40):
+        x, w, b, dh = _gated_inputs(g, M, 24, 16, dtype)
+        far = torch.zeros(M * 2_000_016, device="cuda", dtype=dtype).as_strided((M, 24), (2_000_016, 1))
+        far.copy_(x)
+        out = []
+        for t in (x, far):
+            leaf = t.detach().requires_grad_()
+            h = ops.gated_linear(leaf, w, b)
+            out.append((h.detach(), *torch.autograd.grad(h, leaf, dh)))
+        assert all(torch.equal(p, q) for p, q in zip(*out))
+
+
+def test_parameters_with_strides():
+    """Strided leaves: their gradients, and the refusal to capture beside a living graph of theirs."""
+    g = _gen(48)
+    x, dy = _randn(g, 20, 32), _randn(g, 20, 32)
+    w, b, gw, gb = (t[..., ::2].requires_grad_() for t in (_randn(g, 64), _randn(g, 64), _randn(g, 64, 64), _randn(g, 128)))
+    calls = (lambda w, b: ops.layer_norm(x, w, b), (w, b)), (lambda w, b: ops.gated_linear(x, w, b), (gw, gb))
+    for call, leaves in calls:
+        assert all(t.is_leaf and not t.is_contiguous() for t in leaves)
+        alive = call(*leaves)
+        dense = [t.detach().contiguous().requires_grad_() for t in leaves]
+        want = torch.autograd.grad(call(*dense), dense, dy)
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call(*leaves)
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(alive, leaves, dy), want))
+
+
 def test_refused_on_the_gpu():
     x, w = torch.zeros(3, 4, device="cuda"), torch.zeros(6, 4, device="cuda")
     for bad in (torch.float16, torch.float64):
