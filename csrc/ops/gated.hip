@@ -265,6 +265,16 @@ enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3 };
 // bf16 tiles swap the operands of the matrix instruction, so that a lane holds four neighbouring columns of one row and
 // stages them in LDS with one 8-byte write; fp32 results leave from the accumulators as 128-byte row pieces.
 // KEPT (BWD): the products come from `saved`.
+//
+// Bound by the matrix cores and how well they are fed where K is long.  8192 x 2048 x 8192 bf16: forward 473 us (1.16
+// PFLOP/s; 540 us when it keeps its products: 537 MB written), dx 438 us (1.25), dW 456 us (1.2); a library product of that
+// size reaches 1.45.  The matrix cores are busy 53 - 69 % of the cycles: each SIMD has two waves, and what one waits for at
+// a step's barrier the other hides only in part.  A third set of operands on the way, LDS filled without registers, a
+// workgroup that walks over several tiles and loads that touch the next step's lines ahead were slower or equal.
+// Bound by the epilogue and the latency of a tile where K is short.  25600 x 256 x 1024 bf16 (K = 4 steps, 800 tiles on 256
+// CUs): forward 51 us, backward pair 82 us (of them the products 24, activations 10, stores 10, dh 6), dx and dW 38 us each.
+// The pair from kept products is bound by memory: 8192 x 2048 x 8192, 0.94 GB in 230 - 270 us.
+// fp32 2500 x 257 x 515: forward 29 us, pair 11, dx and dW 26 each: 180 - 360 tiles for 256 CUs.
 template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT = false>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
   typedef Elem<T> E;
@@ -596,7 +606,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
 // Few rows (M <= 16 MF): bound by reading the weights once.  A workgroup takes 16 columns of F and all rows; its 8 waves
 // take the k steps of 32 in turn (512 contiguous bytes of every weight row at a time), weights and rows straight from
 // memory into v_mfma_f32_16x16x32_bf16 fragments, and add their sums in LDS in order.  Rows and columns past the ends
-// repeat the last one: their results are not stored.
+// repeat the last one: their results are not stored.  8 x 2048 x 8192: 14 us (67 MB of weights, 4.8 TB/s); 1 x 256 x 1024:
+// 4.2 us (latency).
 template <int MF, int ACT>
 __global__ __launch_bounds__(512) void rows_kernel(const bf16* x, long ldx, const bf16* w, long ldw, Bias bias, bf16* h, int M,
                                                    int K, long F) {
@@ -654,7 +665,7 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* src, long lds_, T* ds
   }
 }
 
-// out[i] = sum over the splits' partial results, in a fixed order.
+// out[i] = sum over the splits' partial results, in a fixed order (16 of 2048 x 256: 6.7 us, 5.2 TB/s).
 __global__ __launch_bounds__(256) void splits_kernel(const float* slabs, long slab, int splits, long n, void* out, int out_bf) {
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
     float s = 0.f;
@@ -723,7 +734,9 @@ static void launch(TileArgs g, int splits, hipStream_t s) {
   check_launch();
 }
 
-// Rows of a product's tiles (M x N results, bn columns to 256 rows): 256 where those fill the CUs, 128 otherwise, and for
+// Rows of a product's tiles (M x N results, bn columns to 256 rows): 256 where those fill the CUs (forward of 8192 x 2048 x
+// 8192 bf16: 486 us, 613 us on 128 rows), 128 otherwise (dW of 25600 x 256 x 1024 in splits: 39 + 7 us, on 256 rows 44 +
+// 12 us in 31 splits, 49 + 7 us in 16), and for
 // fp32 64 where 128 x 128 tiles leave CUs idle (a step of one keeps a CU's matrix cores 4096 cycles; dx and dW of
 // 2500 x 120 x 520: 30 us on 128 rows, 19 us on 64; large products need the larger tiles' reuse: 64 x 64 alone would read
 // 9 TB/s).
@@ -735,12 +748,13 @@ static int pair_rows(int bf, long M, long F) { return tile_rows(bf, M, F, 128); 
 // Partial rows of the bias gradient: two wave rows a tile.
 static long part_rows(int bf, long M, long F) { return 2 * tiles(M, pair_rows(bf, M, F)); }
 
-// Most rows of the few-rows kernel.
+// Most rows of the few-rows kernel (2048 x 8192 bf16, it and the tiles: 8 rows 13 and 21 us, 32 rows 18 and 20, 64 rows 26
+// and 21).
 constexpr long kRows = 32;
 
 // Whether the forward pass keeps its products: 8 bytes a result written and read again at 4.7 TB/s against 4 D operations
 // at 1.15 PFLOP/s (bf16) or 0.13 (fp32): from D = 1,000 or 110.  (8192 x 2048 x 8192: backward pair 557 us recomputing,
-// 230 us from the kept products, forward 473 -> 546 us; 25600 x 256 x 1024: 90 us recomputing.)
+// 230 - 270 us from the kept products, forward 473 -> 540 us; 25600 x 256 x 1024: 82 us recomputing, 210 MB kept.)
 static bool saves(int bf, long M, long D) { return D >= (bf ? 1024 : 128) && !(bf && M <= kRows); }
 
 // fp32 elements of the kept products, 0 where nothing is kept.
