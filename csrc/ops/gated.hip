@@ -275,19 +275,26 @@ enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3 };
 // CUs): forward 51 us, backward pair 82 us (of them the products 24, activations 10, stores 10, dh 6), dx and dW 38 us each.
 // The pair from kept products is bound by memory: 8192 x 2048 x 8192, 0.94 GB in 230 - 270 us.
 // fp32 2500 x 257 x 515: forward 29 us, pair 11, dx and dW 26 each: 180 - 360 tiles for 256 CUs.
-template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT = false>
-__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
-  typedef Elem<T> E;
-  constexpr int WAVES = WM * WN, NT = 64 * WAVES, BM = 32 * RM * WM, BN = 32 * RN * WN;
-  constexpr bool PAIR = EPI == FWD || EPI == BWD, SWAP = E::CHUNK == 8 && EPI != SUM;
-  constexpr int BH = PAIR ? BN / 2 : BN;            // columns of one product
-  constexpr int SH = PAIR ? RN / 2 : RN;            // 32-column fragments of one product per wave
-  constexpr int ASZ = BM * E::STEP, BSZ = BN * E::STEP, OPS = KEPT ? 0 : 2 * (ASZ + BSZ) * (int)sizeof(T);
-  constexpr int OC = EPI == FWD ? BH : BN, OLD = OC + 8;   // output columns of the tile, staged row stride
-  constexpr int STG = SWAP ? BM * OLD * 2 : 0;
-  constexpr int USE = OPS > STG ? OPS : STG, BIAS = PAIR ? 2 * BH * 4 : 0;
+template <class T, int RM, int RN, int WM, int WN, int EPI, bool KEPT>
+struct Shape {
+  static constexpr int WAVES = WM * WN, NT = 64 * WAVES, BM = 32 * RM * WM, BN = 32 * RN * WN, STEP = Elem<T>::STEP;
+  static constexpr bool PAIR = EPI == FWD || EPI == BWD, SWAP = Elem<T>::CHUNK == 8 && EPI != SUM;
+  static constexpr int BH = PAIR ? BN / 2 : BN;            // columns of one product
+  static constexpr int SH = PAIR ? RN / 2 : RN;            // 32-column fragments of one product per wave
+  static constexpr int ASZ = BM * STEP, BSZ = BN * STEP, OPS = KEPT ? 0 : 2 * (ASZ + BSZ) * (int)sizeof(T);
+  static constexpr int OC = EPI == FWD ? BH : BN, OLD = OC + 8;   // output columns of the tile, staged row stride
+  static constexpr int STG = SWAP ? BM * OLD * 2 : 0;
+  static constexpr int USE = OPS > STG ? OPS : STG, LDS = USE + (PAIR ? 2 * BH * 4 : 0);   // bytes
   static_assert(!PAIR || 2 * BH <= NT, "a bias element per thread");
-  __shared__ __attribute__((aligned(1024))) char smem[USE + BIAS];
+};
+
+template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT>
+__device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
+  typedef Elem<T> E;
+  typedef Shape<T, RM, RN, WM, WN, EPI, KEPT> S;
+  constexpr int WAVES = S::WAVES, NT = S::NT, BM = S::BM, BN = S::BN, BH = S::BH, SH = S::SH, ASZ = S::ASZ, BSZ = S::BSZ,
+                OC = S::OC, OLD = S::OLD, USE = S::USE;
+  constexpr bool PAIR = S::PAIR, SWAP = S::SWAP;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   // steps of a segment; first and number of this split's, over all segments
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
   Copy<T, BM, WAVES, ACOL> ca;
   Copy<T, BH, WAVES, BCOL> cb;
   int pm, pn;
-  tile_of(blockIdx.x, g.tm, g.tn, pm, pn);
+  tile_of(block, g.tm, g.tn, pm, pn);
   const int up = !PAIR && g.tmh && pm >= g.tmh, part_row = pm * WM + wm;   // up: rows of dW's up half
   if (up) pm -= g.tmh;
   const long m0 = (long)pm * BM, n0 = (long)pn * BH;
@@ -601,6 +608,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
   }
 }
 
+template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(TileArgs g) {
+  __shared__ __attribute__((aligned(1024))) char smem[Shape<T, RM, RN, WM, WN, EPI, KEPT>::LDS];
+  tile<T, RM, RN, WM, WN, ACOL, BCOL, EPI, KEPT>(g, blockIdx.x, smem);
+}
+
+// A pair's rows in two parts: `first` tiles of 256 rows, and tiles of 64 rows behind them in the same launch.
+template <class T, int EPI, bool KEPT>
+__global__ __launch_bounds__(512, 2) void two_part_kernel(TileArgs g, TileArgs tail, int first) {
+  __shared__ __attribute__((aligned(1024))) char smem[Shape<T, 4, 2, 2, 4, EPI, KEPT>::LDS];
+  static_assert(Shape<T, 1, 2, 2, 4, EPI, KEPT>::LDS <= sizeof(smem), "tile");
+  if ((int)blockIdx.x < first) tile<T, 4, 2, 2, 4, false, false, EPI, KEPT>(g, blockIdx.x, smem);
+  else tile<T, 1, 2, 2, 4, false, false, EPI, KEPT>(tail, blockIdx.x - first, smem);
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 
 // Few rows (M <= 16 MF): bound by reading the weights once.  A workgroup takes 16 columns of F and all rows; its 8 waves
@@ -745,8 +767,21 @@ static int tile_rows(int bf, long M, long N, long bn) {
   return bf || tiles(M, 128) * tiles(N, bn / 2) >= cu_count() ? 128 : 64;
 }
 static int pair_rows(int bf, long M, long F) { return tile_rows(bf, M, F, 128); }
+
+// Rows of a bf16 pair in tiles of 256 rows: all, or as many tile rows as fill whole rounds of the CUs, where 64-row tiles of
+// the others fill no more than one: 25600 x 256 x 1024 is 3.1 rounds; forward 51 us in 256-row tiles alone, 48 us in two
+// parts, backward pair 82 and 73 us (128-row tiles behind: 49 and 76 us).
+constexpr long kTail = 64;
+static long full_rows(int bf, long M, long F) {
+  if (!bf || pair_rows(bf, M, F) != 256) return M;
+  const long tm = tiles(M, 256), tn = tiles(F, 128), cus = cu_count(), full = tm * tn / cus * cus / tn;
+  return full < tm && tiles(M - 256 * full, kTail) * tn <= cus ? 256 * full : M;
+}
 // Partial rows of the bias gradient: two wave rows a tile.
-static long part_rows(int bf, long M, long F) { return 2 * tiles(M, pair_rows(bf, M, F)); }
+static long part_rows(int bf, long M, long F) {
+  const long full = full_rows(bf, M, F);
+  return 2 * (tiles(full, pair_rows(bf, M, F)) + tiles(M - full, kTail));
+}
 
 // Most rows of the few-rows kernel (2048 x 8192 bf16, it and the tiles: 8 rows 13 and 21 us, 32 rows 18 and 20, 64 rows 26
 // and 21).
@@ -760,12 +795,37 @@ static bool saves(int bf, long M, long D) { return D >= (bf ? 1024 : 128) && !(b
 // fp32 elements of the kept products, 0 where nothing is kept.
 long saved_elements(int bf, long M, long D, long F) {
   if (!saves(bf, M, D)) return 0;
-  const int r = pair_rows(bf, M, F);
-  return tiles(M, r) * r * tiles(F, r == 256 ? 128 : 64) * (r == 256 ? 256 : 128);
+  const long r = pair_rows(bf, M, F), full = full_rows(bf, M, F);
+  return (tiles(full, r) * r + tiles(M - full, kTail) * kTail) * tiles(F, r == 256 ? 128 : 64) * (r == 256 ? 256 : 128);
+}
+
+// Both parts of a pair in one launch: `full` rows in tiles of 256, the others in tiles of kTail.
+template <int EPI, bool KEPT>
+static void two_parts(TileArgs g, long full, hipStream_t s) {
+  TileArgs tail = g;
+  g.tn = tail.tn = (int)tiles(g.N, 128);
+  g.tm = (int)(full / 256);
+  tail.tm = (int)tiles(g.M - full, kTail);
+  g.M = full;
+  tail.M -= full;
+  g.chunk = tail.chunk = (int)tiles(g.K, Elem<bf16>::STEP);
+  tail.a[0] = reinterpret_cast<const bf16*>(g.a[0]) + full * g.lda;
+  tail.dh = g.dh ? reinterpret_cast<const bf16*>(g.dh) + full * g.lddh : nullptr;
+  tail.out = reinterpret_cast<bf16*>(g.out) + full * g.ldo;
+  tail.part = g.part ? g.part + 2 * (long)g.tm * 2 * g.half : nullptr;
+  tail.saved = g.saved ? g.saved + full * g.tn * 256 : nullptr;
+  const long first = (long)g.tm * g.tn, blocks = first + (long)tail.tm * tail.tn;
+  GSC_CHECK(blocks * 512 <= 0xffffffffL, "gated_linear: too many tiles");
+  hipLaunchKernelGGL((two_part_kernel<bf16, EPI, KEPT>), dim3((unsigned)blocks), dim3(512), 0, s, g, tail, (int)first);
+  check_launch();
 }
 
 template <class T, int EPI, bool KEPT = false>
 static void pair(const TileArgs& g, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    const long full = full_rows(1, g.M, g.N);
+    if (full < g.M) return two_parts<EPI, KEPT>(g, full, s);
+  }
   switch (pair_rows(sizeof(T) == 2, g.M, g.N)) {
     case 256: launch<T, 4, 2, 2, 4, false, false, EPI, KEPT>(g, 1, s); break;
     case 128: launch<T, 2, 2, 2, 2, false, false, EPI, KEPT>(g, 1, s); break;
