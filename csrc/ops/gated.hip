@@ -28,6 +28,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef short s16x8_any __attribute__((ext_vector_type(8), aligned(2)));   // at any element's alignment
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(bf16 v) { return __bfloat162float(v); }
@@ -457,7 +458,7 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
     }
     if constexpr (KEPT) __syncthreads();   // the biases are stored
   }
-  // bf16 backward: the tile of dh passes through registers
+  // bf16 backward: the tile of dh passes through registers, in 16-byte pieces at any alignment (rows may end inside one)
   constexpr int DPT = EPI == BWD && SWAP ? BM * BH / 8 / NT : 1;
   s16x8 dh[DPT];
   if constexpr (EPI == BWD && SWAP) {
@@ -465,8 +466,16 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
     for (int q = 0; q < DPT; ++q) {
       const int idx = q * NT + tid, row = idx / (BH / 8), c = idx % (BH / 8) * 8;
       dh[q] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (m0 + row < g.M && n0 + c < g.N)
-        dh[q] = *reinterpret_cast<const s16x8*>(reinterpret_cast<const short*>(g.dh) + (m0 + row) * g.lddh + n0 + c);
+      if (m0 + row < g.M && n0 + c < g.N) {
+        const short* p = reinterpret_cast<const short*>(g.dh) + (m0 + row) * g.lddh + n0 + c;
+        const int left = (int)min(g.N - n0 - c, 8L);
+        if (left == 8) {
+          dh[q] = *reinterpret_cast<const s16x8_any*>(p);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 7; ++e) dh[q][e] = e < left ? p[min(e, left - 1)] : (short)0;
+        }
+      }
     }
   }
   if constexpr (!SWAP) {
@@ -677,13 +686,14 @@ __global__ __launch_bounds__(512) void rows_kernel(const bf16* x, long ldx, cons
     if (f + e < F) h[m * F + f + e] = __float2bfloat16(act_fwd<ACT>(sg[e] + bias.at(f + e)) * (su[e] + bias.at(F + f + e)));
 }
 
-// dst [rows][ldd]: the rows of src, zeros behind them.
+// dst [rows + rows2][ldd]: the rows of src and of src2, zeros behind each.
 template <class T>
-__global__ __launch_bounds__(256) void pad_kernel(const T* src, long lds_, T* dst, long ldd, long rows, long cols) {
-  const long n = rows * ldd;
+__global__ __launch_bounds__(256) void pad_kernel(const T* src, long lds_, long rows, const T* src2, long lds2, long rows2,
+                                                  T* dst, long ldd, long cols) {
+  const long n = (rows + rows2) * ldd;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
     const long r = i / ldd, c = i - r * ldd;
-    dst[i] = c < cols ? src[r * lds_ + c] : T(0.f);
+    dst[i] = c >= cols ? T(0.f) : r < rows ? src[r * lds_ + c] : src2[(r - rows) * lds2 + c];
   }
 }
 
@@ -888,12 +898,17 @@ void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bia
   else pair<float, FWD>(g, stream_of(stream));
 }
 
-void pad(uintptr_t src, long lds_, uintptr_t dst, long ldd, int bf, long rows, long cols, uintptr_t stream) {
-  GSC_CHECK(rows >= 1 && cols >= 1 && cols <= ldd, "gated_linear: pad");
+void pad(uintptr_t src, long lds_, long rows, uintptr_t src2, long lds2, long rows2, uintptr_t dst, long ldd, int bf, long cols,
+         uintptr_t stream) {
+  GSC_CHECK(rows >= 1 && rows2 >= 0 && cols >= 1 && cols <= ldd, "gated_linear: pad");
   const hipStream_t s = stream_of(stream);
-  const dim3 grid(flat_grid(rows * ldd));
-  if (bf) hipLaunchKernelGGL((pad_kernel<bf16>), grid, dim3(256), 0, s, ptr<const bf16>(src), lds_, ptr<bf16>(dst), ldd, rows, cols);
-  else hipLaunchKernelGGL((pad_kernel<float>), grid, dim3(256), 0, s, ptr<const float>(src), lds_, ptr<float>(dst), ldd, rows, cols);
+  auto go = [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL(pad_kernel<T>, dim3(flat_grid((rows + rows2) * ldd)), dim3(256), 0, s, ptr<const T>(src), lds_, rows,
+                       ptr<const T>(src2), lds2, rows2, ptr<T>(dst), ldd, cols);
+  };
+  if (bf) go((bf16*)nullptr);
+  else go((float*)nullptr);
   check_launch();
 }
 
@@ -903,7 +918,6 @@ static void backward_pair(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, 
                    uintptr_t dgu, uintptr_t part, uintptr_t db, int db_bf, uintptr_t saved, long M, long D, long F, int act,
                    uintptr_t stream) {
   TileArgs g = pair_args(x, ldx, w, ldw, bf, bias, bias_bf, M, D, F, act);
-  if (bf) check_operand(dh, lddh);
   const hipStream_t s = stream_of(stream);
   g.dh = ptr<const void>(dh);
   g.lddh = lddh;
@@ -1045,7 +1059,7 @@ void backward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bi
 
 void register_gated(py::module_& m) {
   m.def("gated_forward", &gated::forward, "h = act(x Wg^T + bg) * (x Wu^T + bu)");
-  m.def("gated_pad", &gated::pad, "rows copied to a padded row length, zeros behind them");
+  m.def("gated_pad", &gated::pad, "the rows of two matrices copied to a padded row length, zeros behind them");
   m.def("gated_workspace", &gated::workspace, "bytes of the backward pass's workspace");
   m.def("gated_backward", &gated::backward, "dx, dW and the bias gradient");
   m.def("gated_saved_elements", &gated::saved_elements, "fp32 elements of the products the forward pass keeps (0: none)");

@@ -34,16 +34,27 @@ def gated_linear_reference(x: torch.Tensor, weight: torch.Tensor, bias: Optional
     return (a * u).to(x.dtype)
 
 
-def _operand(t: torch.Tensor) -> torch.Tensor:
-    """The matrix [rows, cols] as the kernels read it: rows start on 16 bytes, at most 2,000,000 elements apart, and end on a
-    multiple of 8 elements (a copy with zeros behind each row where they do not)."""
-    rows, cols = t.shape
-    if rows == 0 or (cols % 8 == 0 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-                     and cols <= t.stride(0) <= 2_000_000):
-        return t
-    out = torch.empty(rows, -(-cols // 8) * 8, device=t.device, dtype=t.dtype)
-    launch(load_native().gated_pad, t, t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0), is_bf16(t), rows, cols)
-    return out
+def _operands(x: torch.Tensor, w: torch.Tensor):
+    """Both matrices as the kernels read them: rows start on 16 bytes, at most 2,000,000 elements apart, and end on a multiple
+    of 8 elements (copies with zeros behind each row where they do not; of both in one launch)."""
+    M, D = x.shape
+    bad = []
+    if M:
+        for t in (x, w):
+            ld = t.stride(0)
+            if D % 8 or ld % 8 or t.data_ptr() % 16 or not D <= ld <= 2_000_000:
+                bad.append(t)
+    if not bad:
+        return x, w
+    a, b = bad[0], bad[1] if len(bad) == 2 else None
+    rows = a.shape[0]
+    rows2, ld2 = (0, 0) if b is None else (b.shape[0], b.stride(0))
+    out = torch.empty(rows + rows2, -(-D // 8) * 8, device=x.device, dtype=x.dtype)
+    launch(load_native().gated_pad, a, a.data_ptr(), a.stride(0), rows, ptr(b), ld2, rows2, out.data_ptr(), out.stride(0),
+           is_bf16(x), D)
+    if b is not None:
+        return out[:rows], out[rows:]
+    return (out, w) if a is x else (x, out)
 
 
 def _forward(x2, w, bias, act, D, saved=None):
@@ -60,7 +71,7 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, w, act, dtype):
         D, bias = x.shape[-1], dense(bias)
-        x2, w = _operand(rows_of(x, D).to(dtype)), _operand(w)
+        x2, w = _operands(rows_of(x, D).to(dtype), w)
         nat, M, Fo, bf = load_native(), x2.shape[0], w.shape[0] // 2, is_bf16(x2)
         n = nat.gated_saved_elements(bf, M, D, Fo) if M else 0
         saved = torch.empty(n, device=x2.device) if n else None
@@ -87,8 +98,7 @@ class _GatedLinear(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
         else:
-            dh2 = rows_of(dh, Fo).to(x2.dtype)
-            dh2 = _operand(dh2) if bf else dh2
+            dh2 = rows_of(dh, Fo)
             work = torch.empty(ctx.space, device=dev, dtype=torch.uint8)
             ctx.run(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), bf, ptr(bias), b_bf, dh2.data_ptr(), dh2.stride(0),
                     ptr(saved), ptr(dx), xt is torch.bfloat16, ptr(dw), wt is torch.bfloat16, ptr(db), bt is torch.bfloat16,
@@ -130,5 +140,5 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         h = _GatedLinear.apply(x, weight, bias, w, ACTIVATIONS[activation], dtype)
         return note_leaves("gated_linear", h, x, weight, bias)
-    h = _forward(_operand(rows_of(x, D).to(dtype)), _operand(w), dense(bias), ACTIVATIONS[activation], D)
+    h = _forward(*_operands(rows_of(x, D).to(dtype), w), dense(bias), ACTIVATIONS[activation], D)
     return h.view(*x.shape[:-1], h.shape[1])
