@@ -213,10 +213,12 @@ struct TileArgs {
   void* out;
   long ldo;
   long half;          // dgu: column of du
-  long slab;          // elements between the fp32 partial results of two splits
+  long slab;          // elements between the fp32 partial results (FWD, PART: accumulators) of two splits
   int tmh;            // dW: tile rows of the gate half (the up half follows), 0 otherwise
   float* part;
   float* saved;       // accumulators of the pair products, [tile][register quarter][thread][4]
+  float* splits;      // the same of each split (FWD, PART)
+  int nsplits;
   int act;
 };
 
@@ -260,12 +262,25 @@ __host__ __device__ __forceinline__ void by_act(int act, F&& finish) {
 }
 
 // What leaves a tile: FWD h, BWD dgu (and the bias gradient's partial sums), OUT the product in T, SUM in fp32 (split
-// partial results, gradients of fp32 masters).
-enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3 };
+// partial results, gradients of fp32 masters), PART a pair's accumulators over a split of K, which a FWD tile adds.
+enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3, PART = 4 };
+
+template <class T, int RM, int RN, int WM, int WN, int EPI, bool KEPT>
+struct Shape {
+  static constexpr int WAVES = WM * WN, NT = 64 * WAVES, BM = 32 * RM * WM, BN = 32 * RN * WN, STEP = Elem<T>::STEP;
+  static constexpr bool PAIR = EPI == FWD || EPI == BWD || EPI == PART, SWAP = Elem<T>::CHUNK == 8 && EPI != SUM;
+  static constexpr int BH = PAIR ? BN / 2 : BN;            // columns of one product
+  static constexpr int SH = PAIR ? RN / 2 : RN;            // 32-column fragments of one product per wave
+  static constexpr int ASZ = BM * STEP, BSZ = BN * STEP, OPS = KEPT ? 0 : 2 * (ASZ + BSZ) * (int)sizeof(T);
+  static constexpr int OC = EPI == FWD ? BH : BN, OLD = OC + 8;   // output columns of the tile, staged row stride
+  static constexpr int STG = SWAP && EPI != PART ? BM * OLD * 2 : 0;
+  static constexpr int USE = OPS > STG ? OPS : STG, LDS = USE + (PAIR ? 2 * BH * 4 : 0);   // bytes
+  static_assert(!PAIR || 2 * BH <= NT, "a bias element per thread");
+};
 
 // bf16 tiles swap the operands of the matrix instruction, so that a lane holds four neighbouring columns of one row and
 // stages them in LDS with one 8-byte write; fp32 results leave from the accumulators as 128-byte row pieces.
-// KEPT (BWD): the products come from `saved`.
+// KEPT: the products come from memory (BWD: those the forward pass kept, FWD: the splits').
 //
 // Bound by the matrix cores and how well they are fed where K is long.  8192 x 2048 x 8192 bf16: forward 473 us (1.16
 // PFLOP/s; 540 us when it keeps its products: 537 MB written), dx 438 us (1.25), dW 456 us (1.2); a library product of that
@@ -273,22 +288,10 @@ enum Epi { FWD = 0, BWD = 1, OUT = 2, SUM = 3 };
 // a step's barrier the other hides only in part.  A third set of operands on the way, LDS filled without registers, a
 // workgroup that walks over several tiles and loads that touch the next step's lines ahead were slower or equal.
 // Bound by the epilogue and the latency of a tile where K is short.  25600 x 256 x 1024 bf16 (K = 4 steps, 800 tiles on 256
-// CUs): forward 51 us, backward pair 82 us (of them the products 24, activations 10, stores 10, dh 6), dx and dW 38 us each.
+// CUs, the last of them in 64-row tiles): forward 48 us, backward pair 73 us (of them the products 24, activations 10, stores
+// 10, dh 6), dx and dW 38 us each.
 // The pair from kept products is bound by memory: 8192 x 2048 x 8192, 0.94 GB in 230 - 270 us.
 // fp32 2500 x 257 x 515: forward 29 us, pair 11, dx and dW 26 each: 180 - 360 tiles for 256 CUs.
-template <class T, int RM, int RN, int WM, int WN, int EPI, bool KEPT>
-struct Shape {
-  static constexpr int WAVES = WM * WN, NT = 64 * WAVES, BM = 32 * RM * WM, BN = 32 * RN * WN, STEP = Elem<T>::STEP;
-  static constexpr bool PAIR = EPI == FWD || EPI == BWD, SWAP = Elem<T>::CHUNK == 8 && EPI != SUM;
-  static constexpr int BH = PAIR ? BN / 2 : BN;            // columns of one product
-  static constexpr int SH = PAIR ? RN / 2 : RN;            // 32-column fragments of one product per wave
-  static constexpr int ASZ = BM * STEP, BSZ = BN * STEP, OPS = KEPT ? 0 : 2 * (ASZ + BSZ) * (int)sizeof(T);
-  static constexpr int OC = EPI == FWD ? BH : BN, OLD = OC + 8;   // output columns of the tile, staged row stride
-  static constexpr int STG = SWAP ? BM * OLD * 2 : 0;
-  static constexpr int USE = OPS > STG ? OPS : STG, LDS = USE + (PAIR ? 2 * BH * 4 : 0);   // bytes
-  static_assert(!PAIR || 2 * BH <= NT, "a bias element per thread");
-};
-
 template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT>
 __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
   typedef Elem<T> E;
@@ -438,26 +441,41 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
 
   // ---- epilogue
   if constexpr (PAIR) {
-    f32x4* kept = reinterpret_cast<f32x4*>(g.saved) + ((long)pm * g.tn + pn) * (RM * RN * 4) * NT + tid;
-    if (KEPT || g.saved) {
+    constexpr int Q = RM * RN * 4;   // four accumulators each
+    const long at = ((long)pm * g.tn + pn) * Q * NT + tid;
+    auto quad = [&](int k) {
+      const f32x16& c = acc[k / 4 / RN][k / 4 % RN];
+      const int e = k % 4 * 4;
+      return f32x4{c[e], c[e + 1], c[e + 2], c[e + 3]};
+    };
+    if constexpr (KEPT) {
+      const f32x4* from = reinterpret_cast<const f32x4*>(EPI == FWD ? g.splits : g.saved) + at;
 #pragma unroll
-      for (int i = 0; i < RM; ++i)
+      for (int k = 0; k < Q; ++k) {
+        const f32x4 v = from[k * NT];
 #pragma unroll
-        for (int j = 0; j < RN; ++j)
+        for (int e = 0; e < 4; ++e) acc[k / 4 / RN][k / 4 % RN][k % 4 * 4 + e] = v[e];
+      }
+      if constexpr (EPI == FWD) {
+        for (int z = 1; z < g.nsplits; ++z) {
+          from += g.slab / 4;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            f32x4& at = kept[((i * RN + j) * 4 + q) * NT];
-            if constexpr (KEPT) {
-              const f32x4 v = at;
+          for (int k = 0; k < Q; ++k) {
+            const f32x4 v = from[k * NT];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e];
-            } else {
-              at = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-            }
+            for (int e = 0; e < 4; ++e) acc[k / 4 / RN][k / 4 % RN][k % 4 * 4 + e] += v[e];
           }
+        }
+      }
+    }
+    float* to = EPI == PART ? g.splits + blockIdx.y * g.slab : EPI == FWD ? g.saved : nullptr;
+    if (to) {
+#pragma unroll
+      for (int k = 0; k < Q; ++k) reinterpret_cast<f32x4*>(to)[at + k * NT] = quad(k);
     }
     if constexpr (KEPT) __syncthreads();   // the biases are stored
   }
+  if constexpr (EPI != PART) {
   // bf16 backward: the tile of dh passes through registers, in 16-byte pieces at any alignment (rows may end inside one)
   constexpr int DPT = EPI == BWD && SWAP ? BM * BH / 8 / NT : 1;
   s16x8 dh[DPT];
@@ -615,6 +633,7 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
       }
     }
   }
+  }
 }
 
 template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT>
@@ -753,7 +772,7 @@ static int cu_count() {
 
 template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT = false>
 static void launch(TileArgs g, int splits, hipStream_t s) {
-  constexpr int BM = 32 * RM * WM, BH = EPI == FWD || EPI == BWD ? 16 * RN * WN : 32 * RN * WN;
+  constexpr int BM = 32 * RM * WM, BH = EPI == SUM || EPI == OUT ? 32 * RN * WN : 16 * RN * WN;
   const long tm = tiles(g.M, BM), tn = tiles(g.N, BH);
   GSC_CHECK((g.tmh ? 2 : 1) * tm * tn * (64 * WM * WN) <= 0xffffffffL, "gated_linear: too many tiles");   // threads of a grid
   if (g.tmh) g.tmh = (int)tm;
@@ -809,6 +828,32 @@ long saved_elements(int bf, long M, long D, long F) {
   return (tiles(full, r) * r + tiles(M - full, kTail) * kTail) * tiles(F, r == 256 ? 128 : 64) * (r == 256 ? 256 : 128);
 }
 
+// Splits of a pair's K where its tiles are few: n of them divide the steps of a tile (0.53 us each in bf16, 2.2 or, on 64
+// rows, 1.1 in fp32) by n and cost n times the accumulators of a tile read by one workgroup (0.12 TB/s) and about 6 us for
+// the second launch: the n where both are equal, at least two steps each, and workgroups for two per CU in bf16, for one in
+// fp32 (whose steps are bound by the matrix cores).  100 x 4096 x 256: bf16 34 us unsplit, 21 us split, fp32 145 and 21 us;
+// 512 x 4096 x 1024 bf16 35 and 32 us, fp32 147 and 77 us; not on more than a quarter of the CUs in bf16, where the weights
+// already come at the rate of the memory (200 x 4096 x 8192: 40 us unsplit, 44 us in two).
+static int pair_splits(int bf, long M, long D, long F) {
+  const int r = pair_rows(bf, M, F);
+  const long steps = tiles(up8(D), bf ? 64 : 32), t = tiles(M, r) * tiles(F, 64), cus = cu_count();
+  if (r == 256 || (bf && (M <= kRows || 4 * t > cus))) return 1;
+  const double all = steps * (bf ? 0.53 : r / 64 * 1.1), each = r * 128 * 4 / 0.12e6;
+  const long n = std::min<long>({(long)(std::sqrt(all / each) + 0.5), (bf ? 2 : 1) * cus / t, steps / 2});
+  return n > 1 && all - all / n > 6 + n * each ? (int)tiles(steps, tiles(steps, n)) : 1;
+}
+// fp32 elements of a split's accumulators.
+static long pair_slab(int bf, long M, long F) {
+  const int r = pair_rows(bf, M, F);
+  return tiles(M, r) * r * tiles(F, 64) * 128;
+}
+// fp32 elements of the forward pass's workspace (0: none).
+long forward_space(int bf, long M, long D, long F) {
+  check_sizes(M, D, F, 0);
+  const int n = pair_splits(bf, M, D, F);
+  return n > 1 ? n * pair_slab(bf, M, F) : 0;
+}
+
 // Both parts of a pair in one launch: `full` rows in tiles of 256, the others in tiles of kTail.
 template <int EPI, bool KEPT>
 static void two_parts(TileArgs g, long full, hipStream_t s) {
@@ -832,15 +877,19 @@ static void two_parts(TileArgs g, long full, hipStream_t s) {
 
 template <class T, int EPI, bool KEPT = false>
 static void pair(const TileArgs& g, hipStream_t s) {
-  if constexpr (sizeof(T) == 2) {
+  constexpr bool SPLIT = EPI == PART || (EPI == FWD && KEPT);   // never in 256-row tiles
+  if constexpr (sizeof(T) == 2 && !SPLIT) {
     const long full = full_rows(1, g.M, g.N);
     if (full < g.M) return two_parts<EPI, KEPT>(g, full, s);
   }
+  const int splits = EPI == PART ? g.nsplits : 1;
   switch (pair_rows(sizeof(T) == 2, g.M, g.N)) {
-    case 256: launch<T, 4, 2, 2, 4, false, false, EPI, KEPT>(g, 1, s); break;
-    case 128: launch<T, 2, 2, 2, 2, false, false, EPI, KEPT>(g, 1, s); break;
+    case 256:
+      if constexpr (!SPLIT) launch<T, 4, 2, 2, 4, false, false, EPI, KEPT>(g, 1, s);
+      break;
+    case 128: launch<T, 2, 2, 2, 2, false, false, EPI, KEPT>(g, splits, s); break;
     default:
-      if constexpr (sizeof(T) == 4) launch<T, 1, 2, 2, 2, false, false, EPI, KEPT>(g, 1, s);
+      if constexpr (sizeof(T) == 4) launch<T, 1, 2, 2, 2, false, false, EPI, KEPT>(g, splits, s);
   }
 }
 // The plain products on the same tiles.
@@ -874,8 +923,9 @@ static TileArgs pair_args(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, 
   return g;
 }
 
-void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h, uintptr_t saved,
-             long M, long D, long F, int act, uintptr_t stream) {
+// work: forward_space() elements, or 0 (K is not split).
+void forward_split(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h,
+                   uintptr_t saved, uintptr_t work, long M, long D, long F, int act, uintptr_t stream) {
   TileArgs g = pair_args(x, ldx, w, ldw, bf, bias, bias_bf, M, D, F, act);
   g.out = ptr<void>(h);
   g.ldo = F;
@@ -894,8 +944,22 @@ void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bia
     check_launch();
     return;
   }
-  if (bf) pair<bf16, FWD>(g, stream_of(stream));
-  else pair<float, FWD>(g, stream_of(stream));
+  const hipStream_t s = stream_of(stream);
+  const int n = work ? pair_splits(bf, M, D, F) : 1;
+  if (n > 1) {
+    g.splits = ptr<float>(work);
+    g.nsplits = n;
+    g.slab = pair_slab(bf, M, F);
+    if (bf) pair<bf16, PART>(g, s), pair<bf16, FWD, true>(g, s);
+    else pair<float, PART>(g, s), pair<float, FWD, true>(g, s);
+  } else {
+    if (bf) pair<bf16, FWD>(g, s);
+    else pair<float, FWD>(g, s);
+  }
+}
+void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h, uintptr_t saved,
+             long M, long D, long F, int act, uintptr_t stream) {
+  forward_split(x, ldx, w, ldw, bf, bias, bias_bf, h, saved, 0, M, D, F, act, stream);
 }
 
 void pad(uintptr_t src, long lds_, long rows, uintptr_t src2, long lds2, long rows2, uintptr_t dst, long ldd, int bf, long cols,
@@ -1059,6 +1123,8 @@ void backward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bi
 
 void register_gated(py::module_& m) {
   m.def("gated_forward", &gated::forward, "h = act(x Wg^T + bg) * (x Wu^T + bu)");
+  m.def("gated_forward_split", &gated::forward_split, "the same with a workspace, K split where tiles are few");
+  m.def("gated_forward_space", &gated::forward_space, "fp32 elements of the forward pass's workspace (0: none)");
   m.def("gated_pad", &gated::pad, "the rows of two matrices copied to a padded row length, zeros behind them");
   m.def("gated_workspace", &gated::workspace, "bytes of the backward pass's workspace");
   m.def("gated_backward", &gated::backward, "dx, dW and the bias gradient");

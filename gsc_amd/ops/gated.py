@@ -58,12 +58,13 @@ def _operands(x: torch.Tensor, w: torch.Tensor):
 
 
 def _forward(x2, w, bias, act, D, saved=None):
-    M = x2.shape[0]
-    Fo = w.shape[0] // 2
+    M, Fo, bf, nat = x2.shape[0], w.shape[0] // 2, is_bf16(x2), load_native()
     h = torch.empty(M, Fo, device=x2.device, dtype=x2.dtype)
     if M > 0:
-        launch(load_native().gated_forward, x2, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), is_bf16(x2), ptr(bias),
-               is_bf16(bias), h.data_ptr(), ptr(saved), M, D, Fo, act)
+        n = nat.gated_forward_space(bf, M, D, Fo)
+        work = torch.empty(n, device=x2.device) if n else None
+        launch(nat.gated_forward_split, x2, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), bf, ptr(bias),
+               is_bf16(bias), h.data_ptr(), ptr(saved), ptr(work), M, D, Fo, act)
     return h
 
 

@@ -123,3 +123,14 @@ def test_native_refusals_of_layer_norm_sizes():
         with pytest.raises(RuntimeError, match="layer_norm"):
             nat.LayerNormBackward(True, False, 0, M, C, False, False)
     assert nat.LayerNormBackward(True, False, 0, 1 << 20, 1 << 24, False, False).space <= 1 << 28   # 1 GB
+
+
+def test_forward_workspace_of_gated_linear():
+    """K is split, through a workspace, only where the tiles are few and K is long."""
+    space = pytest.importorskip("gsc_amd.native").load().gated_forward_space
+    assert space(True, 100, 4096, 256) > 0 and space(False, 100, 4096, 256) > 0
+    for sizes in ((1, 4096, 256), (32, 4096, 256), (100, 128, 256), (200, 4096, 8192), (25600, 4096, 1024)):
+        assert space(True, *sizes) == 0
+    assert space(False, 25600, 4096, 1024) == 0
+    with pytest.raises(RuntimeError, match="gated_linear"):
+        space(True, 0, 8, 8)

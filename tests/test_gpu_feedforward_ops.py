@@ -260,7 +260,8 @@ def _blocks_at(groups, seed, offset):
 GATED_SHAPES = [(1, 1, 1), (1, 256, 1024), (2, 8, 5), (3, 100, 33), (8, 512, 96), (16, 64, 64), (33, 72, 40), (64, 22, 256),
                 (65, 257, 129), (100, 64, 256), (130, 96, 200), (257, 264, 136), (300, 31, 77), (600, 320, 512),
                 (1100, 128, 640), (4200, 72, 2101), (4200, 4104, 72), (100, 4104, 2104), (40, 1032, 72),
-                (200, 1100, 130), (2200, 1024, 1100), (90, 128, 64), (8518, 16, 1024), (8518, 1032, 1020)]
+                (200, 1100, 130), (2200, 1024, 1100), (90, 128, 64), (8518, 16, 1024), (8518, 1032, 1020),
+                (33, 4096, 70), (130, 2050, 129), (700, 1500, 60)]
 
 
 def _gated_check(x, w, b, dh, act, op, w_used=None):
