@@ -65,6 +65,22 @@ def test_layer_norm_parameter_types(dtype, wt, bt):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("wt", [BF16, F32])
+@pytest.mark.parametrize("C", [*range(1, 18), 29, 509, 1021, 8187, 16395])
+def test_layer_norm_rows_between_nan(C, dtype, wt):
+    """Rows and parameters that start and end anywhere, with NaN in front of and behind each."""
+    g = _gen(49, C)
+
+    def inside(*shape, t, **kw):
+        out = torch.full((*shape[:-1], C + 11), float("nan"), device="cuda", dtype=t)
+        out[..., 5:5 + C] = _randn(g, *shape, dtype=t, **kw)
+        return out[..., 5:5 + C]
+
+    x, dy = inside(6, C, t=dtype, shift=0.5), inside(6, C, t=dtype)
+    _norm_check(x, inside(C, t=wt, scale=0.2, shift=1.0), inside(C, t=wt, scale=0.2), dy)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("how", ["slice", "odd_slice", "transposed", "three_d", "one_d", "grad_expanded", "x_expanded",
                                  "grad_slice"])
 def test_layer_norm_strides(dtype, how):
