@@ -10,8 +10,9 @@
 // The backward pass keeps the gradient sums of its columns in registers over all rows that a group of lanes takes, adds the
 // groups of a workgroup in LDS and leaves one partial row per workgroup; a second kernel adds those in a fixed order.
 // Bytes read and written a second (a large copy: 4.7 TB/s; the inputs of repeated calls stay in the 256 MB cache):
-//   bf16 16384 x 8192    forward 91 us, 5.9 TB/s   backward 174 us, 4.6 TB/s (sums of the partial rows 12 us of them)
-//   bf16 65536 x 1024    39 us, 6.9                86 us, 4.7          bf16 25600 x 256   7 us, 3.5   10 us, 3.8
+//   bf16 16384 x 8192    forward 91 us, 5.9 TB/s   backward 174 us, 4.6 TB/s (sums of the partial rows 12 us of them);
+//                        inputs from memory: forward 128 us, 4.2 TB/s
+//   bf16 65536 x 1024    39 us, 6.9                86 us, 4.7          bf16 25600 x 256   8 us, 3.3   11 us, 3.6
 //   fp32 32768 x 1023    41 us, 6.6                85 us, 4.7
 #include <hip/hip_bf16.h>
 #include <algorithm>
