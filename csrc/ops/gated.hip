@@ -560,6 +560,7 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
     }
     auto finish = [&](auto act) {
     constexpr int ACT = decltype(act)::value;
+    const long left = g.M - m0 - 32 * wm * RM;   // rows of the matrix from this wave's first on
 #pragma unroll
     for (int j = 0; j < SH; ++j) {
 #pragma unroll
@@ -576,6 +577,7 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
           short* p = stage + (32 * (wm * RM + i) + (lane & 31)) * OLD + col;
           s16x4 v, w;
           if constexpr (EPI == BWD) w = *reinterpret_cast<const s16x4*>(p);
+          const bool in = 32 * i + (lane & 31) < left;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float c = acc[i][j][4 * rg + e];
@@ -584,15 +586,15 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
             } else if constexpr (EPI == FWD) {
               v[e] = to_s(act_fwd<ACT>(c + bg[e]) * (acc[i][j + SH][4 * rg + e] + bu[e]));
             } else {
-              // rows and columns outside have dh = 0
+              // columns outside have dh = 0
               float a, d;
               act_both<ACT>(c + bg[e], a, d);
               const float x = to_f((short)w[e]);
               const float dg = x * (acc[i][j + SH][4 * rg + e] + bu[e]) * d, du = x * a;
               v[e] = to_s(dg);
               w[e] = to_s(du);
-              sg[e] += dg;
-              su[e] += du;
+              sg[e] += in ? dg : 0.f;   // not by dh = 0: a row outside has g, u = 0 w, NaN where w is infinite
+              su[e] += in ? du : 0.f;
             }
           }
           *reinterpret_cast<s16x4*>(p) = v;
