@@ -72,7 +72,7 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, w, act, dtype):
         D, bias = x.shape[-1], dense(bias)
-        x2, w = _operands(rows_of(x, D).to(dtype), w)
+        x2, w = _operands(rows_of(x, D, dtype), w)
         nat, M, Fo, bf = load_native(), x2.shape[0], w.shape[0] // 2, is_bf16(x2)
         n = nat.gated_saved_elements(bf, M, D, Fo) if M else 0
         saved = torch.empty(n, device=x2.device) if n else None
@@ -141,5 +141,5 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         h = _GatedLinear.apply(x, weight, bias, w, ACTIVATIONS[activation], dtype)
         return note_leaves("gated_linear", h, x, weight, bias)
-    h = _forward(*_operands(rows_of(x, D).to(dtype), w), dense(bias), ACTIVATIONS[activation], D)
+    h = _forward(*_operands(rows_of(x, D, dtype), w), dense(bias), ACTIVATIONS[activation], D)
     return h.view(*x.shape[:-1], h.shape[1])

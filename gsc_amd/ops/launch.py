@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import functools
+from typing import Optional
 
 import torch
 from torch.autograd.function import once_differentiable as _once_differentiable
@@ -28,8 +29,11 @@ def is_bf16(t) -> bool:
     return t is not None and t.dtype is torch.bfloat16
 
 
-def rows_of(t: torch.Tensor, C: int) -> torch.Tensor:
-    """[rows, C] view of ``t`` with contiguous rows (a copy only where its strides allow no such view)."""
+def rows_of(t: torch.Tensor, C: int, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """[rows, C] view of ``t`` with contiguous rows (a copy only where its strides allow no such view).  ``dtype``: cast
+    first, since a cast chooses strides of its own (overlapping rows of unit stride come back with others)."""
+    if dtype is not None:
+        t = t.to(dtype)
     t = t if t.dim() == 2 else t.reshape(-1, C)
     return t if C == 1 or t.stride(1) == 1 else t.contiguous()
 

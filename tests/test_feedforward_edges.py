@@ -1,0 +1,18 @@
+"""CPU: what the feed-forward operators do on the host -- row views, refusals, builds."""
+import pytest
+import torch
+
+from gsc_amd.ops.launch import rows_of
+
+
+@pytest.mark.parametrize("view", [lambda t: t.unfold(0, 8, 1)[:5], lambda t: t.unfold(0, 8, 1)[:9], lambda t: t[:40].view(8, 5).t(),
+                                  lambda t: t[:8].expand(5, 8), lambda t: t[:5, None].expand(5, 8),
+                                  lambda t: t.unfold(0, 8, 2)[:6].view(2, 3, 8), lambda t: t[:40].view(5, 8)])
+@pytest.mark.parametrize("dtype", [None, torch.float32, torch.bfloat16])
+def test_rows_are_contiguous_behind_a_cast(view, dtype):
+    """What a kernel reads through (pointer, row stride) are the elements of the view, overlapping windows included."""
+    t = view(torch.arange(64.0))
+    rows = rows_of(t, t.shape[-1], dtype)
+    assert rows.dtype == (dtype or t.dtype) and rows.stride(1) == 1
+    read = torch.as_strided(rows, rows.shape, (rows.stride(0), 1))
+    assert torch.equal(read, t.to(rows.dtype).reshape(-1, t.shape[-1]))

@@ -47,3 +47,20 @@ def test_gated_linear_gradients_with_an_infinite_gate_weight(M, D, dtype):
                                                               torch.ones(M, 1, dtype=torch.float64))
         sel = [F + 3, 2 * F - 1]
         close(name, got[sel].reshape(exact.shape), exact, sums[[3, F - 1]], dtype)
+
+
+@pytest.mark.parametrize("rows", [5, 40])
+def test_gated_linear_casts_overlapping_rows(rows):
+    """fp32 windows of one another's elements under autocast: the cast changes their strides (fewer rows than columns)."""
+    g = torch.Generator().manual_seed(rows)
+    t, w, dh = _randn(g, 80), _randn(g, 48, 24), _randn(g, rows, 24, dtype=BF16)
+    windows = t.unfold(0, 24, 1)[:rows]
+    out = []
+    for x in (windows, windows.contiguous()):
+        with torch.autocast("cuda", dtype=BF16):
+            with torch.no_grad():
+                first = ops.gated_linear(x, w)
+            leaf = w.detach().clone().requires_grad_()
+            h = ops.gated_linear(x, leaf)
+        out.append((first, h.detach(), torch.autograd.grad(h, leaf, dh)[0]))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
