@@ -3,8 +3,8 @@
 //   mu = mean_c x,  r = 1 / sqrt(mean_c (x - mu)^2 + eps),  xh = (x - mu) r,  y = xh w + b
 //   g = dy w,  dx = r (g - mean_c g - xh mean_c(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
 //
-// x, y, dy, dx are bf16 or fp32; w and b fp32 or bf16 each (absent: 1 and 0).  Every sum and statistic is fp32, the variance
-// from the centred values; an output is rounded once.
+// x, y, dy, dx are bf16 or fp32; w and b fp32 or bf16 each (absent: 1 and 0).  Every sum and statistic is fp32, the mean
+// corrected by that of the centred values, the variance from those; an output is rounded once.
 //
 // Bound by memory: a row is read once into registers (G lanes x N pieces of VEC elements), both passes over it run there.
 // The backward pass keeps the gradient sums of its columns in registers over all rows that a group of lanes takes, adds the
@@ -188,11 +188,28 @@ static dim3 grid_of(long blocks) {
   return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
 
+// The mean, corrected by the mean d of x - first, and the mean of the squares about it from q, that about first.  The first
+// one is off by the roundings of a long sum and of 1 / C: of a row of equal values it would leave a difference that 1 / sqrt
+// (eps) makes visible (30000 in 7 columns: 0.5).  Corrected, such a row's mean is its value.  Where the correction is not
+// small beside the spread (again), the difference of the squares' means would cancel: they are summed once more.
+struct Mean {
+  float mu, shift, var;   // shift: mu - first
+  bool again;
+};
+__device__ __forceinline__ Mean corrected(float first, float d, float q) {
+  Mean m;
+  m.mu = first + d;
+  m.shift = m.mu - first;
+  m.var = q - m.shift * (2.f * d - m.shift);
+  m.again = m.shift * m.shift > q * (1.f / 1024.f);
+  return m;
+}
+
 template <class T, int VEC, int G, int N>
 __global__ __launch_bounds__(G > 256 ? G : 256) void fwd_kernel(const T* x, long ldx, Param w, Param b, T* y, float* mean,
                                                                 float* rstd, long M, int C, float eps) {
   constexpr int NT = G > 256 ? G : 256, E = VEC * N;
-  __shared__ float red[2][16];
+  __shared__ float red[4][16];
   const int lane = threadIdx.x % G;
   const long row0 = block_of() * (NT / G) + threadIdx.x / G, row = row0 < M ? row0 : M - 1;
   const T* xr = x + row * ldx;
@@ -213,22 +230,41 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void fwd_kernel(const T* x, long
 #pragma unroll
     for (int e = 0; e < VEC; ++e) s += v[n * VEC + e];
   }
-  const float inv = 1.f / (float)C, mu = group_sum<G>(s, red) * inv;
-  float q = 0.f;
+  const float inv = 1.f / (float)C, first = group_sum<G>(s, red) * inv;
+  float sum[2] = {0.f, 0.f};   // of x - first and its square
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int c = (n * G + lane) * VEC;
     if (c >= C) break;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[n * VEC + e] -= mu;
+    for (int e = 0; e < VEC; ++e) v[n * VEC + e] -= first;
     if (c + VEC > C) {
 #pragma unroll
       for (int e = 1; e < VEC; ++e) v[n * VEC + e] = c + e < C ? v[n * VEC + e] : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) q += v[n * VEC + e] * v[n * VEC + e];
+    for (int e = 0; e < VEC; ++e) {
+      sum[0] += v[n * VEC + e];
+      sum[1] += v[n * VEC + e] * v[n * VEC + e];
+    }
   }
-  const float r = 1.f / sqrtf(group_sum<G>(q, red + 1) * inv + eps);
+  group_sums<G>(sum, red + 1);
+  const Mean m = corrected(first, sum[0] * inv, sum[1] * inv);
+  float var = m.var;
+  if (m.again) {
+    float q = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = (n * G + lane) * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = v[n * VEC + e] - m.shift;
+        q += c + e < C ? d * d : 0.f;
+      }
+    }
+    var = group_sum<G>(q, red + 3) * inv;
+  }
+  const float mu = m.mu, r = 1.f / sqrtf(var + eps);
   if (row0 >= M) return;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -238,7 +274,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void fwd_kernel(const T* x, long
     w.get<VEC>(c, C, 1.f, wv);
     b.get<VEC>(c, C, 0.f, bv);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[n * VEC + e] = v[n * VEC + e] * r * wv[e] + bv[e];
+    for (int e = 0; e < VEC; ++e) v[n * VEC + e] = (v[n * VEC + e] - m.shift) * r * wv[e] + bv[e];
     store<VEC>(y + row * C, c, C, v + n * VEC);
   }
   if (lane == 0 && mean) {
@@ -385,7 +421,7 @@ __device__ __forceinline__ void row_pieces(int C, F&& f) {
 template <class T, int VEC>
 __global__ __launch_bounds__(1024) void fwd_long_kernel(const T* x, long ldx, Param w, Param b, T* y, float* mean,
                                                         float* rstd, long M, int C, float eps) {
-  __shared__ float red[2][16];
+  __shared__ float red[4][16];
   const long row = block_of();
   if (row >= M) return;
   const T* xr = x + row * ldx;
@@ -396,17 +432,34 @@ __global__ __launch_bounds__(1024) void fwd_long_kernel(const T* x, long ldx, Pa
 #pragma unroll
     for (int e = 0; e < VEC; ++e) s += v[e];
   });
-  const float mu = group_sum<1024>(s, red) / (float)C;
-  float q = 0.f;
+  const float inv = 1.f / (float)C, first = group_sum<1024>(s, red) * inv;
+  float sum[2] = {0.f, 0.f};
   row_pieces<VEC>(C, [&](int c, int left) {
     Piece<T, VEC>::get(xr, c, C, v);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float d = e < left ? v[e] - mu : 0.f;
-      q += d * d;
+      const float d = e < left ? v[e] - first : 0.f;
+      sum[0] += d;
+      sum[1] += d * d;
     }
   });
-  const float r = 1.f / sqrtf(group_sum<1024>(q, red + 1) / (float)C + eps);
+  group_sums<1024>(sum, red + 1);
+  const Mean m = corrected(first, sum[0] * inv, sum[1] * inv);
+  const float mu = m.mu;
+  float var = m.var;
+  if (m.again) {
+    float q = 0.f;
+    row_pieces<VEC>(C, [&](int c, int left) {
+      Piece<T, VEC>::get(xr, c, C, v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float d = e < left ? v[e] - mu : 0.f;
+        q += d * d;
+      }
+    });
+    var = group_sum<1024>(q, red + 3) * inv;
+  }
+  const float r = 1.f / sqrtf(var + eps);
   row_pieces<VEC>(C, [&](int c, int) {
     Piece<T, VEC>::get(xr, c, C, v);
     w.get<VEC>(c, C, 1.f, wv);

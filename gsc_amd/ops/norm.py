@@ -21,7 +21,8 @@ def layer_norm_reference(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                          eps: float = 1e-5) -> torch.Tensor:
     """The same function in elementary PyTorch operations (fp32 inside, or fp64 for fp64 inputs), differentiable."""
     xf = x if x.dtype == torch.float64 else x.float()
-    d = xf - xf.mean(-1, keepdim=True)
+    mu = xf.mean(-1, keepdim=True)
+    d = xf - (mu + (xf - mu).mean(-1, keepdim=True))   # the sum's rounding taken out: 0 in a row of equal values
     y = d * torch.rsqrt((d * d).mean(-1, keepdim=True) + eps)
     if weight is not None:
         y = y * weight.to(xf.dtype)

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from gsc_amd import ops
 from gsc_amd.ops.launch import rows_of
 
 
@@ -16,3 +17,12 @@ def test_rows_are_contiguous_behind_a_cast(view, dtype):
     assert rows.dtype == (dtype or t.dtype) and rows.stride(1) == 1
     read = torch.as_strided(rows, rows.shape, (rows.stride(0), 1))
     assert torch.equal(read, t.to(rows.dtype).reshape(-1, t.shape[-1]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float64])
+@pytest.mark.parametrize("C", [1, 2, 7, 15, 30, 41, 320, 1003, 16395])
+def test_layer_norm_of_equal_values_is_the_bias(C, dtype):
+    values = torch.tensor([7.0, 300.0, 30000.0, 0.1, -1 / 3, 1e8, -1e-3, 0.0], dtype=dtype)
+    b = torch.randn(C, generator=torch.Generator().manual_seed(C), dtype=dtype)
+    y = ops.layer_norm(values[:, None].repeat(1, C), torch.full((C,), 2.0, dtype=dtype), b)
+    assert torch.equal(y, b.expand_as(y))

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from gsc_amd import ops
-from tests.feedforward_bounds import close, gated_bounds
+from tests.feedforward_bounds import U, close, gated_bounds, half, wide
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,81 @@ def test_gated_linear_casts_overlapping_rows(rows):
             h = ops.gated_linear(x, leaf)
         out.append((first, h.detach(), torch.autograd.grad(h, leaf, dh)[0]))
     assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+NORM_WIDTHS = [1, 2, 7, 15, 30, 41, 320, 1003, 4095, 8192, 16384, 16395, 40000]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("C", NORM_WIDTHS)
+def test_layer_norm_rows_of_equal_values(C, dtype):
+    """y is the bias, bit for bit, whatever the value and the length of the row; dx = (g - mean g) / sqrt(eps), dw = 0."""
+    g = torch.Generator().manual_seed(C)
+    values = torch.tensor([7.0, 300.0, 30000.0, 0.1, -1 / 3, 1e8, -1e-3, 0.0], dtype=dtype)
+    x = values[:, None].repeat(1, C).cuda().requires_grad_()
+    w, b = (_randn(g, C) + 1).requires_grad_(), _randn(g, C).requires_grad_()
+    dy = _randn(g, len(values), C, dtype=dtype)
+    y = ops.layer_norm(x, w, b)
+    assert torch.equal(y.detach(), b.detach().to(dtype).expand_as(x))
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    gw = wide(dy) * wide(w)
+    r = 1e-5 ** -0.5
+    want = r * (gw - gw.mean(-1, keepdim=True))
+    # a sum of C terms, the mean's factor, eps in fp32, its root and the two products: C + 8 roundings of U
+    tol = (C + 8) * U * r * (gw.abs() + gw.abs().mean(-1, keepdim=True))
+    close("dx", dx, want, tol, dtype)
+    assert not dw.any()
+    close("db", db, wide(dy).sum(0), (len(values) + 1) * U * wide(dy).abs().sum(0), F32)
+
+
+@pytest.mark.parametrize("C", [c for c in NORM_WIDTHS if c > 2])
+@pytest.mark.parametrize("mean", [300.0, 30000.0, -1e6])
+def test_layer_norm_rows_with_a_far_mean(C, mean):
+    """The mean loses its own rounding and no more: U |mean|, not the roundings of a sum of C terms of its size."""
+    g = torch.Generator().manual_seed(C)
+    x, w = _randn(g, 9, C) * 3 + mean, _randn(g, C) + 1
+    X, W = wide(x), wide(w)
+    mu = X.mean(-1, keepdim=True)
+    d = X - mu
+    r = (d.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    # mean: its own rounding and C + 6 of the centred values, which the first estimate moves by at most (C + 2) U |mean|
+    off = (C + 2) * U * abs(mean)
+    emu = U * mu.abs() + (C + 6) * U * (d.abs().mean(-1, keepdim=True) + off)
+    # squares: C + 8 roundings relative to the mean square about the first estimate, below twice the variance where off is
+    # small and summed again where not; half of it in r.  The moved mean adds its square.
+    er = (C + 8) * U + (emu * r).square()
+    want = d * r * W
+    close("y", ops.layer_norm(x, w), want, W.abs() * (r * emu + (d * r).abs() * (er + 4 * U)) + U * want.abs(), F32)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("C", [7, 300, 16395])
+def test_layer_norm_spread_below_the_mean_of_a_long_sum(C, dtype):
+    """One value of a row differs by a step of its type: 1 / std is that of the values, not of the mean's roundings."""
+    step = 2.0 ** (-7 if dtype == BF16 else -23)
+    x = torch.full((3, C), 1.0, dtype=torch.float64)
+    x *= torch.tensor([[30000.0], [1e6], [1.0]]).to(dtype).double()
+    top = 2.0 ** x.log2().floor()
+    x[:, C // 2] += step * top[:, C // 2]
+    x = x.to(dtype).cuda().requires_grad_()
+    X = wide(x)
+    mu = X.mean(-1, keepdim=True)
+    d = X - mu
+    var = d.square().mean(-1, keepdim=True)
+    r = (var + 1e-5).rsqrt()
+    # the kernel's mean is the rounded one: its squares are about that, var + (its error)^2, at most U |mean|
+    g = torch.Generator().manual_seed(C)
+    dy = _randn(g, 3, C, dtype=dtype)
+    (dx,) = torch.autograd.grad(ops.layer_norm(x), x, dy)
+    m32 = mu.float().double()
+    worst = []
+    for m in (m32, torch.nextafter(mu.float(), torch.tensor(1e30)).double(), torch.nextafter(mu.float(), torch.tensor(0.0)).double()):
+        e = X - m
+        rr = (e.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+        G, xh = wide(dy), e * rr
+        want = rr * (G - G.mean(-1, keepdim=True) - xh * (G * xh).mean(-1, keepdim=True))
+        tol = (2 * C + 24) * U * rr * (G.abs() + G.abs().mean(-1, keepdim=True) + xh.abs() * (G * xh).abs().mean(-1, keepdim=True))
+        err = (dx.cpu().double() - want).abs() / (tol + half(dtype) * (want.abs() + tol))
+        worst.append(err.amax(-1))
+    # the mean in fp32 is one of the neighbours of the exact one
+    assert (torch.stack(worst).amin(0) <= 1.0).all(), worst
