@@ -19,7 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_types, dense, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
+from .launch import check_device, check_forward_mode, check_not_traced, check_types, dense, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
 from .linear import shadow
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
@@ -126,6 +126,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         return gated_linear_reference(x, weight, bias, activation)
     check_types("gated_linear", x=x, weight=weight, bias=bias)
     check_device("gated_linear", x, weight=weight, bias=bias, w16=w16)
+    check_forward_mode("gated_linear", x, weight, bias, w16)
     dtype = x.dtype
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
@@ -141,5 +142,6 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         h = _GatedLinear.apply(x, weight, bias, w, ACTIVATIONS[activation], dtype)
         return note_leaves("gated_linear", h, x, weight, bias)
+    check_not_traced("gated_linear")
     h = _forward(*_operands(rows_of(x, D, dtype), w), dense(bias), ACTIVATIONS[activation], D)
     return h.view(*x.shape[:-1], h.shape[1])

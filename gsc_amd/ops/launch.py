@@ -5,6 +5,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable as _once_differentiable
 
 TYPES = (torch.bfloat16, torch.float32)
@@ -53,6 +54,21 @@ def check_types(name: str, **tensors) -> None:
     for k, t in tensors.items():
         if t is not None and t.dtype not in TYPES:
             raise TypeError(f"{name}: {k} must be bfloat16 or float32 on the GPU, got {t.dtype}")
+
+
+def check_forward_mode(name: str, *tensors) -> None:
+    """Refuses inputs with a tangent: a kernel reads the primal alone, and its result would have none."""
+    if forward_ad._current_level < 0:   # no dual level is open
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name}: forward-mode derivatives are not supported on the GPU")
+
+
+def check_not_traced(name: str) -> None:
+    """Refuses a launch under torch.jit.trace: the trace would hold the empty result and not the kernel that fills it."""
+    if torch._C._is_tracing():
+        raise RuntimeError(f"{name}: cannot be traced on the GPU without gradients (the kernel launch is not recorded)")
 
 
 def differentiable_once(backward):

@@ -1,6 +1,7 @@
 """GPU: values at the edges of the feed-forward operators' ranges, against 64-bit results."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from gsc_amd import ops
 from tests.feedforward_bounds import U, close, gated_bounds, half, wide
@@ -142,3 +143,36 @@ def test_layer_norm_spread_below_the_mean_of_a_long_sum(C, dtype):
         worst.append(err.amax(-1))
     # the mean in fp32 is one of the neighbours of the exact one
     assert (torch.stack(worst).amin(0) <= 1.0).all(), worst
+
+
+def _calls(x, w, gw, gb):
+    return {"layer_norm": (lambda **k: ops.layer_norm(**{"x": x, "weight": w, "bias": w, **k}), ("x", "weight", "bias")),
+            "dropout": (lambda **k: ops.dropout(**{"x": x, "p": 0.1, "seed": 1, "residual": x, **k}), ("x", "residual")),
+            "gated_linear": (lambda **k: ops.gated_linear(**{"x": x, "weight": gw, "bias": gb, **k}), ("x", "weight", "bias"))}
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", ["layer_norm", "dropout", "gated_linear"])
+def test_forward_mode_is_refused(name, grad):
+    """A tangent on any input is refused, with and without gradients; inputs without one pass at an open dual level."""
+    g = torch.Generator().manual_seed(1)
+    tensors = _randn(g, 5, 8), _randn(g, 8), _randn(g, 12, 8), _randn(g, 12)
+    call, names = _calls(*tensors)[name]
+    like = dict(zip(("x", "weight", "bias"), (tensors[0], *(tensors[2:] if name == "gated_linear" else (tensors[1],) * 2))),
+                residual=tensors[0])
+    want = call()
+    with forward_ad.dual_level():
+        assert torch.equal(call(), want)
+        for k in names:
+            dual = forward_ad.make_dual(like[k].clone().requires_grad_(grad), torch.ones_like(like[k]))
+            with pytest.raises(NotImplementedError, match=name):
+                call(**{k: dual})
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "dropout", "gated_linear"])
+def test_tracing_without_gradients_is_refused(name):
+    g = torch.Generator().manual_seed(2)
+    x = _randn(g, 5, 8)
+    call, _ = _calls(x, _randn(g, 8), _randn(g, 12, 8), _randn(g, 12))[name]
+    with pytest.raises(RuntimeError, match=f"{name}: cannot be traced"):
+        torch.jit.trace(lambda t: call(x=t), x, check_trace=False)
