@@ -1,9 +1,9 @@
 """Build the in-tree native extension ``gsc_amd/_native*.so`` with hipcc for gfx950.
 
-Every ``.hip``/``.cpp`` under ``csrc/`` is compiled to an object (in parallel, skipped when
-up to date) and linked into one shared library that contains both the host code (CPU simulator
-path, launchers, pybind11 bindings) and the gfx950 code objects.  No torch headers are used:
-kernels take raw device pointers and the current HIP stream, which keeps builds fast.
+Every ``.hip``/``.cpp`` under ``csrc/`` is compiled to an object (in parallel, skipped where the object is
+newer than its sources and was made by the same command) and linked into one shared library that contains
+both the host code (CPU simulator path, launchers, pybind11 bindings) and the gfx950 code objects.  No torch
+headers are used: kernels take raw device pointers and the current HIP stream, which keeps builds fast.
 """
 from __future__ import annotations
 
@@ -85,30 +85,47 @@ def _obj(src: str, sanitize: bool = False) -> str:
     return os.path.join(BUILD + ("_asan" if sanitize else ""), rel + ".o")
 
 
-def _compile(src: str, sanitize: bool = False) -> str:
-    obj = _obj(src, sanitize)
-    newest = max([os.path.getmtime(src)] + [os.path.getmtime(h) for h in _deps(src)])
-    if os.path.exists(obj) and os.path.getmtime(obj) >= newest:
-        return obj
-    cmd = [HIPCC, "-c", src, "-o", obj] + _flags(src) + _includes() + (SAN_COMPILE if sanitize else [])
+def _command(src: str, sanitize: bool = False) -> list:
+    return [HIPCC, "-c", src, "-o", _obj(src, sanitize)] + _flags(src) + _includes() + (SAN_COMPILE if sanitize else [])
+
+
+def _key(out: str, sanitize: bool = False) -> str:
+    """The file that holds the command ``out`` was made by."""
+    return os.path.join(BUILD + ("_asan" if sanitize else ""), os.path.basename(out) + ".cmd")
+
+
+def _make(out: str, inputs, cmd: list, what: str, sanitize: bool, force: bool) -> str:
+    """Runs ``cmd`` unless ``out`` is newer than its inputs and was made by this very command."""
+    key, text = _key(out, sanitize), "\n".join(cmd)
+    if not force and os.path.exists(out) and os.path.exists(key):
+        with open(key) as f:
+            same = f.read() == text
+        if same and os.path.getmtime(out) >= max(os.path.getmtime(i) for i in inputs):
+            return out
+    if os.path.exists(key):
+        os.remove(key)   # a failed or interrupted run leaves no output that looks current
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {src}:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
-    return obj
+        raise RuntimeError(f"{what}:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    with open(key, "w") as f:
+        f.write(text)
+    return out
 
 
-def build(verbose: bool = True, jobs: int = 8, sanitize: bool = False) -> str:
+def _compile(src: str, sanitize: bool = False, force: bool = False) -> str:
+    return _make(_obj(src, sanitize), [src, *_deps(src)], _command(src, sanitize), f"hipcc failed for {src}", sanitize, force)
+
+
+def build(verbose: bool = True, jobs: int = 8, sanitize: bool = False, force: bool = False) -> str:
+    """``force``: compile every source, up to date or not."""
     os.makedirs(BUILD + ("_asan" if sanitize else ""), exist_ok=True)
     srcs = _sources()
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        objs = list(ex.map(lambda s: _compile(s, sanitize), srcs))
+        objs = list(ex.map(lambda s: _compile(s, sanitize, force), srcs))
     out = ext_path(sanitize)
     os.makedirs(os.path.dirname(out), exist_ok=True)
-    if not os.path.exists(out) or os.path.getmtime(out) < max(os.path.getmtime(o) for o in objs):
-        cmd = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", out] + objs + (SAN_LINK if sanitize else [])
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    cmd = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", out] + objs + (SAN_LINK if sanitize else [])
+    _make(out, objs, cmd, "link failed", sanitize, force)
     if verbose:
         print(f"[gsc_amd] native extension: {out}", file=sys.stderr)
     return out

@@ -48,3 +48,41 @@ def test_tangents_and_traces_are_noticed():
 
     with pytest.raises(RuntimeError, match="op: cannot be traced"):
         torch.jit.trace(traced, x)
+
+
+def test_objects_of_another_command_are_compiled_again(tmp_path, monkeypatch):
+    """An object is current when it is newer than its sources and its command line (flags, target, compiler) is the same."""
+    from gsc_amd.native import build as b
+    csrc, ran = tmp_path / "csrc", []
+    csrc.mkdir()
+    (csrc / "a.hip").write_text('#include "a.h"\n')
+    (csrc / "a.h").write_text("\n")
+    (tmp_path / "cc").write_text("#!/bin/sh\nwhile [ $# -gt 1 ]; do [ \"$1\" = -o ] && touch \"$2\"; shift; done\n")
+    (tmp_path / "cc").chmod(0o755)
+    for name, value in (("CSRC", str(csrc)), ("BUILD", str(tmp_path / "obj")), ("HIPCC", str(tmp_path / "cc")),
+                        ("ext_path", lambda sanitize=False: str(tmp_path / "out.so"))):
+        monkeypatch.setattr(b, name, value)
+    run = b.subprocess.run
+    monkeypatch.setattr(b.subprocess, "run", lambda cmd, **k: (ran.append("-c" in cmd), run(cmd, **k))[1])
+
+    def made(**k):
+        ran.clear()
+        b.build(verbose=False, **k)
+        return ran.count(True), ran.count(False)   # compiled, linked
+
+    assert made() == (1, 1) and made() == (0, 0)
+    flags = b._flags
+    monkeypatch.setattr(b, "_flags", lambda src: flags(src) + ["-DX"])
+    assert made()[0] == 1 and made() == (0, 0)
+    monkeypatch.setattr(b, "ARCH", "gfx942")
+    assert made() == (1, 1) and made() == (0, 0)
+    later = (tmp_path / "out.so").stat().st_mtime + 10
+    b.os.utime(csrc / "a.h", (later, later))
+    assert made()[0] == 1
+    b.os.utime(csrc / "a.h", (1, 1))
+    assert made(force=True) == (1, 1) and made() == (0, 0)
+    (tmp_path / "cc").write_text("#!/bin/sh\nexit 1\n")   # a failing compiler leaves nothing current
+    with pytest.raises(RuntimeError, match="hipcc failed"):
+        made(force=True)
+    with pytest.raises(RuntimeError, match="hipcc failed"):
+        made()
