@@ -86,3 +86,13 @@ def test_objects_of_another_command_are_compiled_again(tmp_path, monkeypatch):
         made(force=True)
     with pytest.raises(RuntimeError, match="hipcc failed"):
         made()
+
+
+def test_the_entry_point_compiles_every_source(monkeypatch):
+    import __graft_entry__
+    from gsc_amd.native import build as b
+    seen = []
+    monkeypatch.setattr(b, "build", lambda **k: seen.append(k))
+    pytest.importorskip("gsc_amd.native").load()
+    __graft_entry__.build()
+    assert seen == [{"verbose": True, "force": True}]
