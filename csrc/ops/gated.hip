@@ -39,37 +39,50 @@ __device__ __forceinline__ short to_s(float v) { return __builtin_bit_cast(short
 
 enum Act { SILU = 0, GELU = 1, SIGMOID = 2 };
 
-__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+// FULL (fp32 operands): exponential and reciprocal to an ulp.  bf16 results are rounded to 2^-8 behind them: the hardware's
+// are enough there (relative error of the exponential 2^-24 (|argument| + 2)).
+template <bool FULL>
+__device__ __forceinline__ float exp_of(float x) { return FULL ? expf(x) : __expf(x); }
+template <bool FULL>
+__device__ __forceinline__ float inverse(float x) { return FULL ? 1.f / x : __builtin_amdgcn_rcpf(x); }
 
-// Phi(g) = (1 + erf(g / sqrt 2)) / 2 and e = exp(-g^2 / 2), by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7):
-// the exponential is the one the derivative needs.
+template <bool FULL>
+__device__ __forceinline__ float sigmoid(float g) { return inverse<FULL>(1.f + exp_of<FULL>(-g)); }
+
+// Phi(g) = erfc(-g / sqrt 2) / 2 and e = exp(-g^2 / 2), the exponential that the derivative needs as well.  With z = |g| /
+// sqrt 2 and t = 1 / (1 + 0.4 z), exp(z^2) erfc(z) / 2 = t Q(t): Q is the polynomial of degree 8 of least maximal relative
+// error over |g| <= 14 (6e-8, fitted in 64 bits), so the small values of the negative side are right to their last digits,
+// but for the rounding of g^2 / 2 in the exponent.
+template <bool FULL>
 __device__ __forceinline__ float normal_cdf(float g, float& e) {
-  e = __expf(-0.5f * g * g);
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(g));
-  const float q = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  const float tail = 0.5f * q * e;
+  e = exp_of<FULL>(-0.5f * g * g);
+  const float t = inverse<FULL>(1.f + 0.4f * 0.70710678f * fabsf(g));
+  const float q =
+      0.112817116f + t * (0.113221556f + t * (0.100943796f + t * (0.0966966152f + t * (0.0398782045f + t *
+      (0.0439822488f + t * (0.0419935584f + t * (-0.0701595694f + t * 0.0206265077f)))))));
+  const float tail = t * q * e;
   return g < 0.f ? tail : 1.f - tail;
 }
 
-template <int ACT>
+template <int ACT, bool FULL>
 __device__ __forceinline__ float act_fwd(float g) {
   float e;
-  if (ACT == GELU) return g * normal_cdf(g, e);
-  const float s = sigmoid(g);
+  if (ACT == GELU) return g * normal_cdf<FULL>(g, e);
+  const float s = sigmoid<FULL>(g);
   return ACT == SILU ? g * s : s;
 }
 
 // a = act(g), d = act'(g)
-template <int ACT>
+template <int ACT, bool FULL>
 __device__ __forceinline__ void act_both(float g, float& a, float& d) {
   if (ACT == GELU) {
     float e;
-    const float phi = normal_cdf(g, e);
+    const float phi = normal_cdf<FULL>(g, e);
     a = g * phi;
     d = phi + g * e * 0.39894228f;
     return;
   }
-  const float s = sigmoid(g);
+  const float s = sigmoid<FULL>(g);
   a = ACT == SILU ? g * s : s;
   d = ACT == SILU ? s * (1.f + g * (1.f - s)) : s * (1.f - s);
 }
@@ -518,7 +531,7 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
           if (in && row < left) {
             if constexpr (EPI == BWD) {
               float a, d;
-              act_both<ACT>(acc[i][j][r] + bg, a, d);
+              act_both<ACT, true>(acc[i][j][r] + bg, a, d);
               const float u = acc[i][j + SH][r] + bu;
               const float dg = *dv * u * d, du = *dv * a;
               o[0] = dg;
@@ -526,7 +539,7 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
               sg += dg;
               su += du;
             } else if constexpr (EPI == FWD) {
-              *o = act_fwd<ACT>(acc[i][j][r] + bg) * (acc[i][j + SH][r] + bu);
+              *o = act_fwd<ACT, true>(acc[i][j][r] + bg) * (acc[i][j + SH][r] + bu);
             } else {
               *o = acc[i][j][r];
             }
@@ -584,11 +597,11 @@ __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
             if constexpr (EPI == OUT) {
               v[e] = to_s(c);
             } else if constexpr (EPI == FWD) {
-              v[e] = to_s(act_fwd<ACT>(c + bg[e]) * (acc[i][j + SH][4 * rg + e] + bu[e]));
+              v[e] = to_s(act_fwd<ACT, false>(c + bg[e]) * (acc[i][j + SH][4 * rg + e] + bu[e]));
             } else {
               // columns outside have dh = 0
               float a, d;
-              act_both<ACT>(c + bg[e], a, d);
+              act_both<ACT, false>(c + bg[e], a, d);
               const float x = to_f((short)w[e]);
               const float dg = x * (acc[i][j + SH][4 * rg + e] + bu[e]) * d, du = x * a;
               v[e] = to_s(dg);
@@ -704,7 +717,7 @@ __global__ __launch_bounds__(512) void rows_kernel(const bf16* x, long ldx, cons
   if (m >= M) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (f + e < F) h[m * F + f + e] = __float2bfloat16(act_fwd<ACT>(sg[e] + bias.at(f + e)) * (su[e] + bias.at(F + f + e)));
+    if (f + e < F) h[m * F + f + e] = __float2bfloat16(act_fwd<ACT, false>(sg[e] + bias.at(f + e)) * (su[e] + bias.at(F + f + e)));
 }
 
 // dst [rows + rows2][ldd]: the rows of src and of src2, zeros behind each.

@@ -169,6 +169,7 @@ def test_forward_mode_is_refused(name, grad):
                 call(**{k: dual})
 
 
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
 @pytest.mark.parametrize("name", ["layer_norm", "dropout", "gated_linear"])
 def test_tracing_without_gradients_is_refused(name):
     g = torch.Generator().manual_seed(2)
@@ -176,3 +177,70 @@ def test_tracing_without_gradients_is_refused(name):
     call, _ = _calls(x, _randn(g, 8), _randn(g, 12, 8), _randn(g, 12))[name]
     with pytest.raises(RuntimeError, match=f"{name}: cannot be traced"):
         torch.jit.trace(lambda t: call(x=t), x, check_trace=False)
+
+
+def _activation64(g, act):
+    """act(g), act'(g) in 64 bits, and the sum of the derivative's terms (what its roundings are relative to)."""
+    s = torch.sigmoid(g)
+    if act == "gelu":
+        phi, e = 0.5 * torch.special.erfc(-g * 0.5 ** 0.5), torch.exp(-0.5 * g * g) * (0.5 / torch.pi) ** 0.5
+        return g * phi, phi + g * e, phi + (g * e).abs()
+    c = torch.sigmoid(-g)
+    # 1 - s, of a rounded s, is off by U: two roundings relative to s itself
+    return (g * s, s * (1 + g * c), s * (1 + g.abs() * (c + 1))) if act == "silu" else (s, s * c, s * (c + 1))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [30, 4001])
+def test_activations_are_right_relative_to_their_own_size(rows, dtype, act):
+    """Values and derivatives over g in -12 .. 12, the small ones of the negative side included (up projection 1)."""
+    g = torch.linspace(-12, 12, rows).to(dtype).cuda()
+    x = torch.zeros(rows, 8, device="cuda", dtype=dtype)
+    x[:, 0] = g
+    w, b = torch.zeros(8, 8, device="cuda", dtype=dtype), torch.zeros(8, device="cuda")
+    w[:4, 0] = 1.0      # four gates of x[:, 0]
+    b[4:] = 1.0
+    x.requires_grad_()
+    h = ops.gated_linear(x, w, b, activation=act)
+    dh = torch.zeros_like(h)
+    dh[:, 1] = 1.0
+    (dx,) = torch.autograd.grad(h, x, dh)
+    a, d, size = _activation64(wide(g), act)
+    # exponent: rounding of g^2 / 2 and, in bf16, of its product with log2 e, g^2 U together (|g| U of the others, which is
+    # less than g^2 U + U); exponential, reciprocal and the operations around them 12 U; the polynomial 6.2e-8 < 2 U and its
+    # roundings 3 U
+    rel = (wide(g).square() + 18) * U
+    for k in range(4):
+        close("h", h[:, k], a, rel * a.abs(), dtype)
+    # dg is a matrix operand: rounded to the type once more
+    tol = rel * size
+    close("dx", dx[:, 0], d, tol + (half(dtype) * (d.abs() + tol) if dtype == BF16 else 0), dtype)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("M", [4, 200])
+def test_fp32_activations_of_huge_gates(M, act):
+    """Gates of 1e29: the activation is 0 or the gate itself (sigmoid: 0 or 1), their product with the up projection 0,
+    infinite or the projection."""
+    g = torch.Generator().manual_seed(M)
+    x, w = torch.zeros(M, 100, device="cuda"), _randn(g, 120, 100, scale=0.1)
+    x[:, 0] = 3e30 * torch.where(torch.arange(M, device="cuda") % 2 == 0, 1.0, -1.0)
+    h = ops.gated_linear(x, w, activation=act)
+    gate, up = (wide(x) @ wide(w).t()).chunk(2, 1)
+    on = gate > 0
+    if act == "sigmoid":
+        close("h", h, torch.where(on, up, 0.0), 4 * U * up.abs(), F32)
+    else:
+        assert torch.equal(h.cpu(), torch.where(on, torch.inf * up.sign(), 0.0).float())
+
+
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_fp32_small_values_of_the_sigmoid(act):
+    """Gates down to -80: the exponential's relative error does not grow with its argument."""
+    g = torch.linspace(-80, 0, 4001, device="cuda")
+    x, w = torch.zeros(4001, 8, device="cuda"), torch.zeros(2, 8, device="cuda")
+    x[:, 0], w[0, 0] = g, 1.0
+    h = ops.gated_linear(x, w, torch.tensor([0.0, 1.0], device="cuda"), activation=act)
+    a = _activation64(wide(g), act)[0]
+    close("h", h[:, 0], a, 8 * U * a.abs(), F32)   # exponential, sum, quotient, two products: 8 roundings at most
