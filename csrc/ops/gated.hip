@@ -938,30 +938,29 @@ static TileArgs pair_args(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, 
   return g;
 }
 
-// work: forward_space() elements, or 0 (K is not split).
-void forward_split(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h,
-                   uintptr_t saved, uintptr_t work, long M, long D, long F, int act, uintptr_t stream) {
+// work: n splits' accumulators (n > 1).
+static void run_forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h,
+                        uintptr_t saved, long saved_size, uintptr_t work, int n, long M, long D, long F, int act,
+                        uintptr_t stream) {
   TileArgs g = pair_args(x, ldx, w, ldw, bf, bias, bias_bf, M, D, F, act);
   g.out = ptr<void>(h);
   g.ldo = F;
   g.saved = ptr<float>(saved);
   GSC_CHECK(!saved || saves(bf, M, D), "gated_linear: these products are not kept");
+  GSC_CHECK(!saved || saved_size >= saved_elements(bf, M, D, F), "gated_linear: too little space for the kept products");
+  const hipStream_t s = stream_of(stream);
   if (bf && M <= kRows) {
     by_act<true>(act, [&](auto a) {
       constexpr int ACT = decltype(a)::value;
       auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3((unsigned)tiles(F, 16)), dim3(512), 0, stream_of(stream), ptr<const bf16>(x), ldx,
+        hipLaunchKernelGGL(kern, dim3((unsigned)tiles(F, 16)), dim3(512), 0, s, ptr<const bf16>(x), ldx,
                            ptr<const bf16>(w), ldw, g.bias, ptr<bf16>(h), (int)M, (int)g.K, F);
       };
       if (M <= 16) go(rows_kernel<1, ACT>);
       else go(rows_kernel<2, ACT>);
     });
     check_launch();
-    return;
-  }
-  const hipStream_t s = stream_of(stream);
-  const int n = work ? pair_splits(bf, M, D, F) : 1;
-  if (n > 1) {
+  } else if (n > 1) {
     g.splits = ptr<float>(work);
     g.nsplits = n;
     g.slab = pair_slab(bf, M, F);
@@ -972,9 +971,21 @@ void forward_split(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr
     else pair<float, FWD>(g, s);
   }
 }
+// Without gradients, K in one piece.
 void forward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h, uintptr_t saved,
              long M, long D, long F, int act, uintptr_t stream) {
-  forward_split(x, ldx, w, ldw, bf, bias, bias_bf, h, saved, 0, M, D, F, act, stream);
+  GSC_CHECK(!saved, "gated_linear: this forward pass keeps no products");
+  run_forward(x, ldx, w, ldw, bf, bias, bias_bf, h, 0, 0, 0, 1, M, D, F, act, stream);
+}
+// Keeps its products in saved (saved_size elements; 0: does not) and splits K through work (work_size elements, at least
+// forward_space()).
+void forward_split(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t h,
+                   uintptr_t saved, long saved_size, uintptr_t work, long work_size, long M, long D, long F, int act,
+                   uintptr_t stream) {
+  const long need = forward_space(bf, M, D, F);
+  GSC_CHECK(!need || (work && work_size >= need), "gated_linear: too little workspace for the forward pass");
+  run_forward(x, ldx, w, ldw, bf, bias, bias_bf, h, saved, saved_size, work, need ? pair_splits(bf, M, D, F) : 1, M, D, F, act,
+              stream);
 }
 
 void pad(uintptr_t src, long lds_, long rows, uintptr_t src2, long lds2, long rows2, uintptr_t dst, long ldd, int bf, long cols,
@@ -1122,12 +1133,15 @@ long workspace(int bf, long M, long D, long F, bool need_x, bool need_w, bool ne
   return space_of(bf, M, D, F, need_x, need_w, need_b).size;
 }
 
-// dx, dw, db (0: not asked for) from x, the weights, dh and the kept products (0: computed again).
+// dx, dw, db (0: not asked for) from x, the weights, dh and the kept products (saved_size elements; 0: computed again), in
+// work_size bytes of workspace.
 void backward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bias, int bias_bf, uintptr_t dh, long lddh,
-              uintptr_t saved, uintptr_t dx, int dx_bf, uintptr_t dw, int dw_bf, uintptr_t db, int db_bf, uintptr_t work,
-              long M, long D, long F, int act, uintptr_t stream) {
-  GSC_CHECK(work, "gated_linear: the backward pass needs a workspace");
+              uintptr_t saved, long saved_size, uintptr_t dx, int dx_bf, uintptr_t dw, int dw_bf, uintptr_t db, int db_bf,
+              uintptr_t work, long work_size, long M, long D, long F, int act, uintptr_t stream) {
+  check_sizes(M, D, F, act);
   const Space sp = space_of(bf, M, D, F, dx != 0, dw != 0, db != 0);
+  GSC_CHECK(work && work_size >= sp.size, "gated_linear: too little workspace for the backward pass");
+  GSC_CHECK(!saved || saved_size >= saved_elements(bf, M, D, F), "gated_linear: too few kept products");
   const uintptr_t dgu = work, slabs = work + sp.slabs;
   backward_pair(x, ldx, w, ldw, bf, bias, bias_bf, dh, lddh, dgu, work + sp.part, db, db_bf, saved, M, D, F, act, stream);
   if (dx) backward_x(dgu, w, ldw, bf, dx, dx_bf, slabs, M, D, F, stream);
@@ -1138,7 +1152,7 @@ void backward(uintptr_t x, long ldx, uintptr_t w, long ldw, int bf, uintptr_t bi
 
 void register_gated(py::module_& m) {
   m.def("gated_forward", &gated::forward, "h = act(x Wg^T + bg) * (x Wu^T + bu)");
-  m.def("gated_forward_split", &gated::forward_split, "the same with a workspace, K split where tiles are few");
+  m.def("gated_forward_split", &gated::forward_split, "the same, products kept for the backward pass, K split through a workspace");
   m.def("gated_forward_space", &gated::forward_space, "fp32 elements of the forward pass's workspace (0: none)");
   m.def("gated_pad", &gated::pad, "the rows of two matrices copied to a padded row length, zeros behind them");
   m.def("gated_workspace", &gated::workspace, "bytes of the backward pass's workspace");

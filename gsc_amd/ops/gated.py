@@ -19,7 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_forward_mode, check_not_traced, check_types, dense, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
+from .launch import check_device, check_forward_mode, check_not_traced, check_types, dense, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of, size
 from .linear import shadow
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
@@ -62,9 +62,12 @@ def _forward(x2, w, bias, act, D, saved=None):
     h = torch.empty(M, Fo, device=x2.device, dtype=x2.dtype)
     if M > 0:
         n = nat.gated_forward_space(bf, M, D, Fo)
-        work = torch.empty(n, device=x2.device) if n else None
-        launch(nat.gated_forward_split, x2, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), bf, ptr(bias),
-               is_bf16(bias), h.data_ptr(), ptr(saved), ptr(work), M, D, Fo, act)
+        args = (x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), bf, ptr(bias), is_bf16(bias), h.data_ptr(), ptr(saved))
+        if saved is None and not n:
+            launch(nat.gated_forward, x2, *args, M, D, Fo, act)
+        else:
+            work = torch.empty(n, device=x2.device) if n else None
+            launch(nat.gated_forward_split, x2, *args, size(saved), ptr(work), n, M, D, Fo, act)
     return h
 
 
@@ -102,8 +105,8 @@ class _GatedLinear(torch.autograd.Function):
             dh2 = rows_of(dh, Fo)
             work = torch.empty(ctx.space, device=dev, dtype=torch.uint8)
             ctx.run(x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), bf, ptr(bias), b_bf, dh2.data_ptr(), dh2.stride(0),
-                    ptr(saved), ptr(dx), xt is torch.bfloat16, ptr(dw), wt is torch.bfloat16, ptr(db), bt is torch.bfloat16,
-                    work.data_ptr(), M, D, Fo, act, raw_stream(ctx.dev))
+                    ptr(saved), size(saved), ptr(dx), xt is torch.bfloat16, ptr(dw), wt is torch.bfloat16, ptr(db),
+                    bt is torch.bfloat16, work.data_ptr(), ctx.space, M, D, Fo, act, raw_stream(ctx.dev))
         return dx.view(shape) if dx is not None else None, dw, db, None, None, None
 
 

@@ -26,6 +26,10 @@ def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def size(t) -> int:
+    return 0 if t is None else t.numel()
+
+
 def is_bf16(t) -> bool:
     return t is not None and t.dtype is torch.bfloat16
 

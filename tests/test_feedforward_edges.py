@@ -96,3 +96,39 @@ def test_the_entry_point_compiles_every_source(monkeypatch):
     pytest.importorskip("gsc_amd.native").load()
     __graft_entry__.build()
     assert seen == [{"verbose": True, "force": True}]
+
+
+def test_workspaces_of_other_sizes_are_refused():
+    """On the host, before any launch: the pointers are never read."""
+    nat = pytest.importorskip("gsc_amd.native").load()
+    M, D, F = 100, 4096, 256
+    need, kept = nat.gated_forward_space(True, M, D, F), nat.gated_saved_elements(True, M, D, F)
+    back = nat.gated_workspace(True, M, D, F, True, True, True)
+    assert need > 0 and kept > 0
+
+    def forward(saved, saved_size, work, work_size, sizes=(M, D, F)):
+        nat.gated_forward_split(256, D, 256, D, True, 0, False, 256, saved, saved_size, work, work_size, *sizes, 0, 0)
+
+    for work, work_size in ((0, 0), (0, need), (256, need - 1), (256, nat.gated_forward_space(True, M - 40, D, F) // 2)):
+        with pytest.raises(RuntimeError, match="too little workspace for the forward pass"):
+            forward(256, kept, work, work_size)
+    with pytest.raises(RuntimeError, match="too little space for the kept products"):
+        forward(256, kept - 1, 256, need)
+    with pytest.raises(RuntimeError, match="not kept"):
+        forward(256, 1 << 40, 256, 1 << 40, (M, 64, F))
+    with pytest.raises(RuntimeError, match="keeps no products"):
+        nat.gated_forward(256, D, 256, D, True, 0, False, 256, 256, M, D, F, 0, 0)
+
+    def backward(saved, saved_size, work, work_size, act=0):
+        nat.gated_backward(256, D, 256, D, True, 0, False, 256, F, saved, saved_size, 256, True, 256, True, 256, True, work,
+                           work_size, M, D, F, act, 0)
+
+    for work, work_size in ((0, back), (256, back - 1)):
+        with pytest.raises(RuntimeError, match="too little workspace for the backward pass"):
+            backward(256, kept, work, work_size)
+    with pytest.raises(RuntimeError, match="too few kept products"):
+        backward(256, kept - 1, 256, back)
+    with pytest.raises(RuntimeError, match="kept products"):
+        backward(0, 0, 256, back)
+    with pytest.raises(RuntimeError, match="activation"):
+        backward(256, kept, 256, back, act=3)
