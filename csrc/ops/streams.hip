@@ -25,8 +25,10 @@ static uintptr_t create_cu_masked_stream(std::vector<int> cus) {
   }
   hipStream_t s = nullptr;
   const hipError_t e = hipExtStreamCreateWithCUMask(&s, (uint32_t)mask.size(), mask.data());
-  if (e != hipSuccess) (void)hipGetLastError();  // the caller may go on with another mask
-  GSC_HIP_CHECK(e);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();  // the caller may go on with another mask
+    throw std::runtime_error(std::string("hipExtStreamCreateWithCUMask: ") + hipGetErrorString(e));
+  }
   return reinterpret_cast<uintptr_t>(s);
 }
 

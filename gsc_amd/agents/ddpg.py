@@ -609,14 +609,7 @@ class BatchedTrainer:
                 k = max(8, min(int(sim_cus), n - 8))
                 self.sim_cus = k
                 small_env = (160 * 1024) // max(int(sim.ctx.lds_per_env), 1) >= 4
-                sim_list = self.sim_cu_list(n, k, spread_default=small_env)
-                try:
-                    handle = nat.create_cu_masked_stream(sim_list)
-                except RuntimeError:
-                    # some drivers refuse a spread mask of fewer than 8 bits per 32-bit block (it leaves XCDs without a
-                    # CU); contiguous bits are dealt to the XCDs in turn
-                    sim_list = list(range(k))
-                    handle = nat.create_cu_masked_stream(sim_list)
+                handle, sim_list = self.sim_stream_on(nat, n, k, small_env)
                 rest = [c for c in range(n) if c not in set(sim_list)]
                 self.sim_stream = torch.cuda.ExternalStream(handle, device=self.device)
                 # The learner stream is restricted to the complement, so no learner wave shares a SIMD
@@ -679,6 +672,24 @@ class BatchedTrainer:
             per = k // (n // 32)
             return [c for c in range(n) if c % 32 < per]
         return list(range(k))
+
+    @classmethod
+    def sim_stream_on(cls, nat, n: int, k: int, spread_default: bool):
+        """A stream on ``k`` of ``n`` CUs, and their mask bits.
+
+        Some drivers refuse a spread mask of fewer than 8 bits per 32-bit block (it leaves XCDs without a CU).  Where the
+        layout was not chosen by hand (``GSC_SIM_CU_LAYOUT``), such a mask gives way, with a warning, to contiguous bits,
+        which are dealt to the XCDs in turn.  Any other failure is the caller's."""
+        bits = cls.sim_cu_list(n, k, spread_default=spread_default)
+        try:
+            return nat.create_cu_masked_stream(bits), bits
+        except RuntimeError as e:
+            few = bits != list(range(k)) and k < 8 * (n // 32)
+            if not few or os.environ.get("GSC_SIM_CU_LAYOUT", "auto") != "auto" or "hipExtStreamCreateWithCUMask" not in str(e):
+                raise
+            warnings.warn(f"simulator stream: the driver refuses {k} CUs spread over the XCDs ({e}); using CUs 0 .. {k - 1}")
+            bits = list(range(k))
+            return nat.create_cu_masked_stream(bits), bits
 
     @staticmethod
     def auto_sim_cus(sim) -> int:
