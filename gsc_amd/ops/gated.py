@@ -19,7 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_forward_mode, check_not_traced, check_types, dense, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of, size
+from .launch import check_device, check_forward_mode, check_leaves, check_not_traced, check_types, dense, differentiable_once, is_bf16, launch, ptr, raw_stream, rows_of, size
 from .linear import shadow
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
@@ -143,8 +143,8 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         w = w if w is not None else weight.detach().to(dtype)
     w = rows_of(w.detach(), D)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        h = _GatedLinear.apply(x, weight, bias, w, ACTIVATIONS[activation], dtype)
-        return note_leaves("gated_linear", h, x, weight, bias)
+        check_leaves("gated_linear", x, weight, bias)
+        return _GatedLinear.apply(x, weight, bias, w, ACTIVATIONS[activation], dtype)
     check_not_traced("gated_linear")
     h = _forward(*_operands(rows_of(x, D, dtype), w), dense(bias), ACTIVATIONS[activation], D)
     return h.view(*x.shape[:-1], h.shape[1])

@@ -7,6 +7,7 @@ from typing import Optional
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable as _once_differentiable
+from torch.autograd.graph import get_gradient_edge
 
 TYPES = (torch.bfloat16, torch.float32)
 raw_stream = torch._C._cuda_getCurrentRawStream
@@ -90,23 +91,59 @@ def differentiable_once(backward):
     return run
 
 
-_STREAM = "gsc_amd.stream"
+class _Seen(Exception):
+    pass
 
 
-def note_leaves(name: str, out: torch.Tensor, *inputs) -> torch.Tensor:
-    """Refuses to capture an op on a leaf whose gradient node lives in a graph made on another stream.
+class _NoGradient(torch.autograd.Function):
+    """The identity, whose backward pass hands on no gradient."""
+
+    @staticmethod
+    def forward(ctx, t):
+        return t.view_as(t)
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+def _held(t: torch.Tensor) -> bool:
+    """Whether any graph holds the gradient node of leaf ``t``: a mark on it outlives this function's own reference."""
+    get_gradient_edge(t).node.metadata["gsc_amd.held"] = True
+    return get_gradient_edge(t).node.metadata.pop("gsc_amd.held", False)
+
+
+def _node_stream(t: torch.Tensor):
+    """The stream of leaf ``t``'s gradient node (None: not found).  The engine makes it current before a node's hooks run; the
+    hook ends the pass there.  Without a gradient to hand on, the pass touches no stream, so a capture is left as it was."""
+    if t._backward_hooks:   # they would be called without a gradient
+        return None
+    seen = []
+
+    def look(grads):
+        seen.append(raw_stream(t.get_device()))
+        raise _Seen
+
+    hook = get_gradient_edge(t).node.register_prehook(look)
+    try:
+        torch.autograd.backward([_NoGradient.apply(t)], [t.detach()])
+    except _Seen:
+        pass
+    finally:
+        hook.remove()
+    return seen[0] if seen else None
+
+
+def check_leaves(name: str, *inputs) -> None:
+    """Refuses to capture an op on a leaf whose gradient node lives in a graph made on another stream, by whatever operator.
 
     Autograd keeps one gradient node per leaf for as long as any graph holds it, bound to the stream it was made on.  A
     backward pass captured later would make that stream, outside the capture, wait for the captured one, which ends the
-    process when the capture ends.  ``inputs``: the Function's tensor arguments in order (None: absent)."""
-    nodes = None
-    for i, t in enumerate([t for t in inputs if t is not None]):
-        if not (t.requires_grad and t.is_leaf):
-            continue
-        if nodes is None:
-            nodes, stream = out.grad_fn.next_functions, raw_stream(out.get_device())
-        if (nodes[i][0].metadata.setdefault(_STREAM, stream) != stream and torch.cuda.is_current_stream_capturing()):
+    process when the capture ends."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    for t in inputs:
+        if t is not None and t.requires_grad and t.is_leaf and _held(t) and _node_stream(t) != raw_stream(t.get_device()):
             raise RuntimeError(f"{name}: a graph of the same leaf tensor {tuple(t.shape)}, made on another stream, is still "
                                "alive; a captured backward pass cannot share its gradient node (drop the outputs of "
                                "earlier calls before the capture, or capture with leaves of its own)")
-    return out

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_forward_mode, check_not_traced, check_types, dense, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream, rows_of
+from .launch import check_device, check_forward_mode, check_leaves, check_not_traced, check_types, dense, differentiable_once, is_bf16, launch, ptr, raw_stream, rows_of
 
 
 def layer_norm_reference(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -99,6 +99,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     check_forward_mode("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return note_leaves("layer_norm", _LayerNorm.apply(x, weight, bias, float(eps)), x, weight, bias)
+        check_leaves("layer_norm", x, weight, bias)
+        return _LayerNorm.apply(x, weight, bias, float(eps))
     check_not_traced("layer_norm")
     return _forward(rows_of(x, C), dense(weight), dense(bias), float(eps), False)[0].view(x.shape)

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from gsc_amd.native import load as load_native
-from .launch import check_device, check_forward_mode, check_not_traced, check_types, differentiable_once, is_bf16, launch, note_leaves, ptr, raw_stream
+from .launch import check_device, check_forward_mode, check_leaves, check_not_traced, check_types, differentiable_once, is_bf16, launch, ptr, raw_stream
 
 _M32 = np.uint64(0xFFFFFFFF)
 
@@ -120,7 +120,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
     check_device("dropout", x, residual=residual)
     check_forward_mode("dropout", x, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return note_leaves("dropout", _Dropout.apply(x, residual, float(p), int(seed), int(offset), at), x, residual)
+        check_leaves("dropout", x, residual)
+        return _Dropout.apply(x, residual, float(p), int(seed), int(offset), at)
     check_not_traced("dropout")
     return _launch(x.contiguous(), residual.contiguous() if residual is not None else None, float(p), int(seed),
                    int(offset), at, None)

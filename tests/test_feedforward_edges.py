@@ -1,10 +1,13 @@
 """CPU: what the feed-forward operators do on the host -- row views, refusals, builds."""
+import sys
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from gsc_amd import ops
-from gsc_amd.ops.launch import check_forward_mode, check_not_traced, rows_of
+from gsc_amd.ops import launch
+from gsc_amd.ops.launch import check_forward_mode, check_leaves, check_not_traced, rows_of
 
 
 @pytest.mark.parametrize("view", [lambda t: t.unfold(0, 8, 1)[:5], lambda t: t.unfold(0, 8, 1)[:9], lambda t: t[:40].view(8, 5).t(),
@@ -132,3 +135,33 @@ def test_workspaces_of_other_sizes_are_refused():
         backward(0, 0, 256, back)
     with pytest.raises(RuntimeError, match="activation"):
         backward(256, kept, 256, back, act=3)
+
+
+def test_leaves_held_by_graphs_of_another_stream(monkeypatch):
+    """While capturing: a leaf that any operator's graph holds is refused unless that graph's stream is the captured one."""
+    node, here, capturing = 5, 5, True
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    # the hook in the node asks for its stream, the check for the captured one
+    monkeypatch.setattr(launch, "raw_stream", lambda dev: node if sys._getframe(1).f_code.co_name == "look" else here)
+    w, x = torch.randn(3, requires_grad=True), torch.randn(3)
+    check_leaves("op", x, None, w)               # no graph
+    alive = w * 2
+    check_leaves("op", x, None, w)               # a graph of this stream
+    node = 6
+    with pytest.raises(RuntimeError, match="op: a graph of the same leaf"):
+        check_leaves("op", x, None, w)
+    assert w.grad is None and torch.equal(torch.autograd.grad(alive, w, x, retain_graph=True)[0], 2 * x)   # left as it was
+    check_leaves("op", alive)                    # not a leaf
+    capturing = False
+    check_leaves("op", w)
+    capturing = True
+    del alive
+    check_leaves("op", w)
+    called = []
+    handle = w.register_hook(called.append)
+    check_leaves("op", w)
+    alive = w * 2
+    with pytest.raises(RuntimeError, match="op: a graph"):   # its hooks are not called to find out
+        check_leaves("op", w)
+    assert not called
+    handle.remove()

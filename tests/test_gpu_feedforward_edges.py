@@ -244,3 +244,35 @@ def test_fp32_small_values_of_the_sigmoid(act):
     h = ops.gated_linear(x, w, torch.tensor([0.0, 1.0], device="cuda"), activation=act)
     a = _activation64(wide(g), act)[0]
     close("h", h[:, 0], a, 8 * U * a.abs(), F32)   # exponential, sum, quotient, two products: 8 roundings at most
+
+
+def test_capture_beside_a_graph_of_another_operator():
+    """A living graph of the same leaf is noticed whatever operator made it: refused where it belongs to another stream,
+    not where it is part of the capture itself."""
+    g = torch.Generator().manual_seed(3)
+    x, nw, gw = _randn(g, 20, 32), (_randn(g, 32) + 1).requires_grad_(), _randn(g, 16, 32).requires_grad_()
+    calls = {"norm": (lambda: ops.layer_norm(x, nw), nw), "gated": (lambda: ops.gated_linear(x, gw), gw),
+             "dropout": (lambda: ops.dropout(gw, 0.5, 1, 1), gw)}
+    for call, leaf in calls.values():
+        alive = leaf * 2
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        assert torch.equal(torch.autograd.grad(alive.sum(), leaf)[0], torch.full_like(leaf, 2.0))
+        del alive
+
+        def both():
+            twice = leaf * 2               # holds the leaf's node before the operator sees it
+            y = call()
+            return torch.autograd.grad((twice.sum(), y), leaf, (None, torch.ones_like(y)))[0]
+
+        want = both()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = both()
+        for _ in range(3):
+            got.zero_()
+            gr.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            assert torch.equal(both(), want)
