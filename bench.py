@@ -59,6 +59,13 @@ PRESETS = {
 }
 
 
+def own_model(agent_config: str, learner) -> str:
+    """The networks of an ``--agent-config`` that is not the preset's."""
+    from gsc_amd.models import count_params
+    return (f"GSC DDPG, {os.path.basename(agent_config)}: actor {count_params(learner.actor):,} params, "
+            f"critic {count_params(learner.critic):,} params")
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
@@ -211,7 +218,7 @@ def main():
             **({"diagnostic": "GSC_SIM_PROFILE=1: cycle-counting simulator variant, not a benchmark number"}
                if diag else {}),
             "config": {
-                "model": pre["model"],
+                "model": pre["model"] if agent_config == pre["agent_config"] else own_model(agent_config, trainer.learner),
                 "global_batch": trainer.batch_size * info.world_size,
                 "seq_len": sim.episode_steps,
                 "parallelism": f"dp{info.world_size}",
