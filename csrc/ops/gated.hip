@@ -843,24 +843,28 @@ long saved_elements(int bf, long M, long D, long F) {
   return (tiles(full, r) * r + tiles(M - full, kTail) * kTail) * tiles(F, r == 256 ? 128 : 64) * (r == 256 ? 256 : 128);
 }
 
-// Splits of a pair's K where its tiles are few: n of them divide the steps of a tile (0.53 us each in bf16, 2.2 or, on 64
-// rows, 1.1 in fp32) by n and cost n times the accumulators of a tile read by one workgroup (0.12 TB/s) and about 6 us for
-// the second launch: the n where both are equal, at least two steps each, and workgroups for two per CU in bf16, for one in
-// fp32 (whose steps are bound by the matrix cores).  100 x 4096 x 256: bf16 34 us unsplit, 21 us split, fp32 145 and 21 us;
-// 512 x 4096 x 1024 bf16 35 and 32 us, fp32 147 and 77 us; not on more than a quarter of the CUs in bf16, where the weights
-// already come at the rate of the memory (200 x 4096 x 8192: 40 us unsplit, 44 us in two).
-static int pair_splits(int bf, long M, long D, long F) {
-  const int r = pair_rows(bf, M, F);
-  const long steps = tiles(up8(D), bf ? 64 : 32), t = tiles(M, r) * tiles(F, 64), cus = cu_count();
-  if (r == 256 || (bf && (M <= kRows || 4 * t > cus))) return 1;
-  const double all = steps * (bf ? 0.53 : r / 64 * 1.1), each = r * 128 * 4 / 0.12e6;
-  const long n = std::min<long>({(long)(std::sqrt(all / each) + 0.5), (bf ? 2 : 1) * cus / t, steps / 2});
-  return n > 1 && all - all / n > 6 + n * each ? (int)tiles(steps, tiles(steps, n)) : 1;
-}
 // fp32 elements of a split's accumulators.
 static long pair_slab(int bf, long M, long F) {
   const int r = pair_rows(bf, M, F);
   return tiles(M, r) * r * tiles(F, 64) * 128;
+}
+
+// Splits of a pair's K where its tiles are few: n of them divide the steps of a tile (0.53 us each in bf16, 2.2 or, on 64
+// rows, 1.1 in fp32) by n and cost n times the accumulators of a tile read by one workgroup (0.12 TB/s), n times all of them
+// written and read (4.7 TB/s) and about 6 us for the second launch: the n where both are equal, at least two steps each, and
+// workgroups for two per CU in bf16, for one in fp32 (whose steps are bound by the matrix cores); not on more than a quarter
+// of the CUs in bf16, where the weights already come at the rate of the memory.  In one piece and as called:
+//   100 x 4096 x 256    bf16 34 us, 20 (7 pieces)   fp32 146, 23      512 x 4096 x 1024   bf16 36 us, 25 (4)   fp32 155, 90
+//   64 x 2048 x 512     bf16 19 us, 14              fp32 74, 18       300 x 2048 x 1024   bf16 20 us, not split (23 in 6)
+//   128 x 8192 x 512    bf16 64 us, 30              fp32 288, 43      200 x 4096 x 8192   bf16 41 us, not split (44 in 2)
+static int pair_splits(int bf, long M, long D, long F) {
+  const int r = pair_rows(bf, M, F);
+  const long steps = tiles(up8(D), bf ? 64 : 32), t = tiles(M, r) * tiles(F, 64), cus = cu_count();
+  if (r == 256 || (bf && (M <= kRows || 4 * t > cus))) return 1;
+  const double all = steps * (bf ? 0.53 : r / 64 * 1.1);
+  const double each = r * 128 * 4 / 0.12e6 + pair_slab(bf, M, F) * 8 / 4.7e6;
+  const long n = std::min<long>({(long)(std::sqrt(all / each) + 0.5), (bf ? 2 : 1) * cus / t, steps / 2});
+  return n > 1 && all - all / n > 6 + n * each ? (int)tiles(steps, tiles(steps, n)) : 1;
 }
 // fp32 elements of the forward pass's workspace (0: none).
 long forward_space(int bf, long M, long D, long F) {
