@@ -276,3 +276,10 @@ def test_capture_beside_a_graph_of_another_operator():
             torch.cuda.synchronize()
             assert torch.equal(got, want)
             assert torch.equal(both(), want)
+
+
+@pytest.mark.parametrize("B", [100, 25600])
+def test_graphed_updates_of_the_trained_batches(B):
+    """The batches of one and of 256 environments: replays equal eager updates, library reductions in the graph included."""
+    from tests.test_gpu_feedforward_learner import test_graphed_updates_equal_eager_ones
+    test_graphed_updates_equal_eager_ones(B)
