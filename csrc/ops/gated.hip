@@ -4,7 +4,10 @@
 //   forward     both products of a tile in one kernel; bias, activation, product and rounding in its epilogue
 //   backward    g and u from the fp32 accumulators again -- kept by the forward pass, or computed once more where that
 //               is cheaper (saves()) -- dg = dh u act'(g), du = dh act(g), rounded once to the operand type;
-//               dx = dg Wg + du Wu,  dW = [dg | du]^T x,  db = column sums (fp32)
+//               dx = dg Wg + du Wu,  dW = [dg | du]^T x,  db = column sums (fp32, of the unrounded values)
+// The rounding of dg and du to bf16 operands is the one besides the results' own: a norm error of 0.0023 in dx and dW against
+// 64 bits, 0.0017 without it (25600 x 256 x 1024).  More bits would need a second product of the remainders, twice the time
+// of dx and dW; fp32 operands keep them.
 //
 // bf16 operands run on v_mfma_f32_32x32x16_bf16, fp32 on v_mfma_f32_32x32x2_f32.
 #include <hip/hip_bf16.h>
@@ -295,16 +298,17 @@ struct Shape {
 // stages them in LDS with one 8-byte write; fp32 results leave from the accumulators as 128-byte row pieces.
 // KEPT: the products come from memory (BWD: those the forward pass kept, FWD: the splits').
 //
-// Bound by the matrix cores and how well they are fed where K is long.  8192 x 2048 x 8192 bf16: forward 473 us (1.16
-// PFLOP/s; 540 us when it keeps its products: 537 MB written), dx 438 us (1.25), dW 456 us (1.2); a library product of that
-// size reaches 1.45.  The matrix cores are busy 53 - 69 % of the cycles: each SIMD has two waves, and what one waits for at
-// a step's barrier the other hides only in part.  A third set of operands on the way, LDS filled without registers, a
-// workgroup that walks over several tiles and loads that touch the next step's lines ahead were slower or equal.
-// Bound by the epilogue and the latency of a tile where K is short.  25600 x 256 x 1024 bf16 (K = 4 steps, 800 tiles on 256
-// CUs, the last of them in 64-row tiles): forward 48 us, backward pair 73 us (of them the products 24, activations 10, stores
-// 10, dh 6), dx and dW 38 us each.
-// The pair from kept products is bound by memory: 8192 x 2048 x 8192, 0.94 GB in 230 - 270 us.
-// fp32 2500 x 257 x 515: forward 29 us, pair 11, dx and dW 26 each: 180 - 360 tiles for 256 CUs.
+// Bound by the matrix cores and how well they are fed where K is long.  8192 x 2048 x 8192 bf16: forward 464 us (gelu,
+// 1.18 PFLOP/s; silu 447; 545 - 554 us when it keeps its products: 537 MB written), dx 438 us (1.25), dW 449 us (1.2); a
+// library product of that size reaches 1.45.  The matrix cores are busy 52 - 66 % of the cycles: each SIMD has two waves,
+// and what one waits for at a step's barrier the other hides only in part.  A third set of operands on the way, LDS
+// filled without registers, a workgroup that walks over several tiles and loads that touch the next step's lines ahead
+// were slower or equal.
+// Bound by the epilogue and the latency of a tile where K is short.  25600 x 256 x 1024 bf16 (K = 4 steps, 800 tiles on
+// 256 CUs, the last of them in 64-row tiles): forward 47 us (gelu 51), backward pair 73 us (gelu 78; of them the products
+// 24, silu and its derivative 10, stores 10, dh 6), dx and dW 38 us each.
+// The pair from kept products is bound by memory: 8192 x 2048 x 8192, 0.94 GB in 265 - 272 us.
+// fp32 2500 x 257 x 515: forward 29 us, pair 12, dx and dW 24 - 26 each: 180 - 360 tiles for 256 CUs.
 template <class T, int RM, int RN, int WM, int WN, bool ACOL, bool BCOL, int EPI, bool KEPT>
 __device__ __forceinline__ void tile(const TileArgs& g, int block, char* smem) {
   typedef Elem<T> E;
@@ -833,7 +837,7 @@ constexpr long kRows = 32;
 
 // Whether the forward pass keeps its products: 8 bytes a result written and read again at 4.7 TB/s against 4 D operations
 // at 1.15 PFLOP/s (bf16) or 0.13 (fp32): from D = 1,000 or 110.  (8192 x 2048 x 8192: backward pair 557 us recomputing,
-// 230 - 270 us from the kept products, forward 473 -> 540 us; 25600 x 256 x 1024: 82 us recomputing, 210 MB kept.)
+// 270 us from the kept products, forward 464 -> 545 us; 25600 x 256 x 1024: 82 us recomputing, 210 MB kept.)
 static bool saves(int bf, long M, long D) { return D >= (bf ? 1024 : 128) && !(bf && M <= kRows); }
 
 // fp32 elements of the kept products, 0 where nothing is kept.

@@ -9,11 +9,12 @@
 // Bound by memory: a row is read once into registers (G lanes x N pieces of VEC elements), both passes over it run there.
 // The backward pass keeps the gradient sums of its columns in registers over all rows that a group of lanes takes, adds the
 // groups of a workgroup in LDS and leaves one partial row per workgroup; a second kernel adds those in a fixed order.
-// Bytes read and written a second (a large copy: 4.7 TB/s; the inputs of repeated calls stay in the 256 MB cache):
-//   bf16 16384 x 8192    forward 91 us, 5.9 TB/s   backward 174 us, 4.6 TB/s (sums of the partial rows 12 us of them);
-//                        inputs from memory: forward 128 us, 4.2 TB/s
-//   bf16 65536 x 1024    39 us, 6.9                86 us, 4.7          bf16 25600 x 256   8 us, 3.3   11 us, 3.6
-//   fp32 32768 x 1023    41 us, 6.6                85 us, 4.7
+// Repeated calls, bytes read and written a second (a large copy: 4.7 TB/s; what fits the 256 MB cache stays there), and of the
+// backward's time that of the partial rows' sums:
+//   bf16 16384 x 8192    forward 121 us, 4.4 TB/s   backward 176 - 185 us, 4.5 TB/s (sums 12)
+//   bf16 65536 x 1024    40 us, 6.7                 85 us, 4.7 (5)          bf16 25600 x 256   6.5 us, 4.0   15 us, 2.6 (4)
+//   fp32 32768 x 1023    42 us, 6.4                 85 us, 4.7 (6)
+// The correction of the mean costs 3 - 5 % of a wide row's forward pass (16384 x 8192: 118 us without), nothing elsewhere.
 #include <hip/hip_bf16.h>
 #include <algorithm>
 #include <pybind11/pybind11.h>
@@ -35,7 +36,7 @@ __device__ __forceinline__ unsigned bits(bf16 v) { return __builtin_bit_cast(uns
 // any element's alignment: rows of odd lengths start anywhere.  The last piece of a row is read VEC elements before the
 // row's end and shifted, so nothing outside the row is touched; elements past the end are 0.  Loading and unpacking are two
 // steps, so that a caller sends all its loads first.  (16384 x 8192 bf16 off 16-byte alignment, element by element: forward
-// 297 us, backward 480 us; in pieces 96 and 171 us, on aligned rows 91 and 174 us.)  VEC 1: rows shorter than a piece.
+// 297 us, backward 480 us; in pieces 143 and 170 us, on aligned rows 121 and 180 us.)  VEC 1: rows shorter than a piece.
 template <class T, int VEC>
 struct Piece {
   static constexpr int D = VEC == 1 ? 1 : VEC * (int)sizeof(T) / 4;
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, sizeof(T) == 2 ? 4 : 2) void bwd
 }
 
 // ---- rows too long for registers: three passes over a row by a workgroup, column sums by a kernel of their own.  All but
-// the first pass read what the caches hold (8192 rows of bf16: 16,384 columns in registers 92 and 202 us, 16,392 so 117 and
+// the first pass read what the caches hold (8192 rows of bf16: 16,384 columns in registers 128 and 203 us, 16,392 so 160 and
 // 341 us).
 
 // f(c, left): the pieces of a row that this thread of 1024 takes, and how many of a piece's elements are inside.

@@ -5,7 +5,9 @@
 ``gated_linear`` runs both projections, the activation and the product in one HIP kernel for CUDA tensors, and
 :func:`gated_linear_reference` otherwise.  Operands are bf16 or fp32 with fp32 accumulation.  The backward pass takes every
 derivative from the fp32 values of both projections: it computes them again from ``x``, or, from ``D`` = 1,024 (bf16) or 128
-(fp32) on, where that costs more than memory, reads what the forward pass kept (8 bytes for each element of ``h``).
+(fp32) on, where that costs more than memory, reads what the forward pass kept (8 bytes for each element of ``h``; a caller
+short of memory between the passes recomputes the layer with ``torch.utils.checkpoint``).  Second derivatives, forward-mode derivatives and
+traces without gradients are refused on the GPU.
 
 * bf16 ``x`` with fp32 masters: the weight operand is the masters' bf16 shadow (``FlatParams``) or a cast; their gradients
   come back in fp32.  Under autocast fp32 ``x`` is cast the same way, like :func:`gsc_amd.ops.linear.linear`.

@@ -5,7 +5,8 @@
 ``layer_norm`` runs the HIP kernels for CUDA tensors and :func:`layer_norm_reference` otherwise.  ``x`` is bf16 or fp32,
 of any shape; ``weight`` and ``bias`` [C] are each fp32, bf16 or absent, whatever the type of ``x`` (bf16 activations
 with the learner's fp32 masters need no cast).  Statistics and sums are fp32, ``y`` and the gradients have the types of
-``x``, ``weight`` and ``bias``; the parameter gradients are summed in a fixed order (bitwise reproducible).
+``x``, ``weight`` and ``bias``; the parameter gradients are summed in a fixed order (bitwise reproducible).  Second
+derivatives, forward-mode derivatives and traces without gradients are refused on the GPU.
 """
 from __future__ import annotations
 
@@ -83,7 +84,8 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
-    """See the module docstring.  ``eps`` > 0 keeps rows of equal values finite (their ``y`` is ``bias``)."""
+    """See the module docstring.  ``eps`` > 0 keeps rows of equal values finite (their ``y`` is ``bias``); the sum of a
+    row has to stay in the range of fp32."""
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"layer_norm: x needs a last dimension of at least 1, got shape {tuple(x.shape)}")
     C = x.shape[-1]

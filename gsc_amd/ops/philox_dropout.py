@@ -6,7 +6,8 @@ GPU, on the CPU and for any strides: callers give every call site its own ``seed
 
 ``offset`` is an int, or a one-element int64 CUDA tensor read when the kernel runs: in a captured HIP graph each replay
 draws a new mask once something in (or between) the replays has advanced that tensor.  The forward call keeps the value
-it read for its own backward pass, so the tensor may be advanced between the two.
+it read for its own backward pass, so the tensor may be advanced between the two.  Second derivatives, forward-mode
+derivatives and traces without gradients are refused on the GPU.
 """
 from __future__ import annotations
 
